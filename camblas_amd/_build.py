@@ -51,6 +51,7 @@ CORE_SOURCES = (
     "routing.hip", "dense_ops.hip", "sgemm_mfma.hip", "dgemm_mfma.hip", "strassen.hip",
     "fusion.hip",
     "attention_decode.hip",
+    "abi_paged.hip", "paged_append.hip", "paged_decode.hip", "paged_prefill.hip",
 )
 
 HIP_FLAGS = [

@@ -35,7 +35,14 @@ _ALGORITHMS = ALGORITHMS
 COUNTERS = ("classical", "strassen", "gram", "affine", "lt", "guard_fallback", "attention", "backward")
 
 _P, _I, _F, _D, _C = ct.c_void_p, ct.c_int, ct.c_float, ct.c_double, ct.c_char
-_U64, _SZ = ct.c_uint64, ct.c_size_t
+_U64, _SZ, _L = ct.c_uint64, ct.c_size_t, ct.c_int64
+
+
+class PagedCache(ct.Structure):
+    """camblas_cuda_paged_cache: where the pages of a key-value cache lie (strides in elements)."""
+
+    _fields_ = [("k", _P), ("v", _P), ("page_stride", _L), ("slot_stride", _L), ("head_stride", _L), ("pages", _I),
+                ("page_size", _I), ("kv_heads", _I), ("dim", _I)]
 
 
 def _gemm(scalar):
@@ -93,6 +100,10 @@ SIGNATURES = {
     "bf16_rms_gated_linear": ([_P, _I, _I, _I, _P, _I, _P, _I, _I, _P, _F, _P, _P, _I, _P, _I], _I),
     "add_residual_squares": ([_P, _I, _I, _P, _P, _P, _P], _I),
     "fp8_moe_decode": ([_P, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _F, _P], _I),
+    "qk_norm_rope_append": ([_P, _I, _I, _I, _F, _I, _F, _P, _P, _P, _P, _P, _L, _P, _L, _P], _I),
+    "paged_decode_workspace_size": ([_P, _I, _I, _P, _I, _I, _I], _SZ),
+    "paged_decode_attention": ([_P, _I, _I, _P, _P, _L, _I, _P, _I, _I, _F, _P, _L, _P, _SZ, _P, _L], _I),
+    "paged_prefill_attention": ([_P, _I, _I, _I, _P, _P, _L, _I, _P, _P, _I, _I, _F, _P, _L, _P, _L], _I),
     "hip_plan_describe": ([_I, _I, _C, _C, _I, _I, _I, _I, _I, _I, _I, ct.c_char_p, _SZ], _I),
     "hip_set_plan_override": ([_P, _I, _I], _I),
     "hip_kernel_count": ([_I], _I),

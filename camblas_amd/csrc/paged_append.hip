@@ -1,0 +1,201 @@
+// What a decoder layer does with a fused QKV activation before attention over a paged cache, in one
+// launch: the RMS norm of every query and key head (optional), the rotary embedding, the queries into
+// their output, keys and values into their slots.
+//
+//   y = x * rsqrt(mean(x^2) + epsilon) * weight          over one head's dims
+//   (lo, hi) -> (lo cos a - hi sin a, hi cos a + lo sin a)   lo = y[i], hi = y[i + rotary / 2],
+//                                                        a = position * theta^(-2 i / rotary)
+//
+// All of it in FP32 with one rounding to BF16 at the end. The angle is formed in FP64 as a number of
+// turns, of which the whole ones are dropped before the FP32 sine and cosine: at position 2^20 an angle
+// in FP32 is off by up to 2^-4 of a radian.
+//
+// A lane owns eight pairs of a head: dims 8 j .. 8 j + 7 and rotary / 2 further (dims that are not
+// rotated are dealt in the same way: two runs of eight), so dim / 16 lanes hold a head, the sum of squares
+// stays within them and the angles of a lane are the same for every head of a token. A wavefront takes
+// some or all heads of one token.
+#include "common.hpp"
+#include "device.hpp"
+#include "paged_cache.hpp"
+
+#include <cmath>
+
+namespace camblas_hip
+{
+namespace
+{
+constexpr int APPEND_WAVES = 4;
+
+struct AppendParams {
+    int tokens, q_heads, parts, groups_per_part;
+    int half; // rotary / 2
+    float epsilon;
+    const void *q_weight, *k_weight; // null: no norm
+    int weight_bf16;
+    const int32_t *positions;
+    const int64_t *slots;
+    const unsigned short *qkv;
+    unsigned short *q_out;
+    int64_t token_stride, out_stride;
+    PagedCache cache;
+    double turns[64]; // theta^(-2 i / rotary) / (2 pi)
+};
+
+__device__ __forceinline__ void load_weights(const void *weight, int bf16, int at, float (&w)[8])
+{
+    if (bf16) {
+        const u32x4_t packed = *reinterpret_cast<const u32x4_t *>(static_cast<const unsigned short *>(weight) + at);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            w[2 * e] = __uint_as_float(packed[e] << 16);
+            w[2 * e + 1] = __uint_as_float(packed[e] & 0xffff0000u);
+        }
+    } else {
+        const float *from = static_cast<const float *>(weight) + at;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            w[e] = from[e];
+    }
+}
+
+__device__ __forceinline__ void unpack(const u32x4_t &packed, float (&x)[8])
+{
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        x[2 * e] = __uint_as_float(packed[e] << 16);
+        x[2 * e + 1] = __uint_as_float(packed[e] & 0xffff0000u);
+    }
+}
+
+__device__ __forceinline__ u32x4_t pack(const float (&x)[8])
+{
+    return u32x4_t{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7])};
+}
+
+template <int DIM> __global__ __launch_bounds__(APPEND_WAVES * 64) void qk_norm_rope_append_kernel(AppendParams p)
+{
+    constexpr int LANES = DIM / 16, HEADS = 64 / LANES; // lanes of a head, heads a wavefront takes at once
+    const int lane = threadIdx.x % 64;
+    const int64_t index = int64_t(blockIdx.x) * APPEND_WAVES + threadIdx.x / 64;
+    const int token = int(index / p.parts), part = int(index % p.parts);
+    if (token >= p.tokens)
+        return;
+    const int j = lane % LANES, rotating = p.half / 8; // lanes of a head whose dims are rotated
+    const bool rotates = j < rotating;
+    const int low = rotates ? 8 * j : 2 * p.half + 16 * (j - rotating);
+    const int high = rotates ? low + p.half : low + 8;
+    const int kv_heads = p.cache.kv_heads, heads = p.q_heads + 2 * kv_heads;
+
+    const double position = double(p.positions[token]);
+    float s[8], c[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const double turn = position * p.turns[rotates ? 8 * j + e : 0];
+        sincospif(2.f * float(turn - rint(turn)), &s[e], &c[e]);
+        if (!rotates) {
+            s[e] = 0.f;
+            c[e] = 1.f;
+        }
+    }
+    float q_low[8], q_high[8], k_low[8], k_high[8];
+    if (p.q_weight) {
+        load_weights(p.q_weight, p.weight_bf16, low, q_low);
+        load_weights(p.q_weight, p.weight_bf16, high, q_high);
+        load_weights(p.k_weight, p.weight_bf16, low, k_low);
+        load_weights(p.k_weight, p.weight_bf16, high, k_high);
+    }
+    const int64_t slot = p.slots[token];
+    const int64_t page = slot >> p.cache.page_shift;
+    const bool stored = slot >= 0 && page < p.cache.pages;
+    const int64_t row = stored ? row_offset(p.cache, int(page), int(slot & ((int64_t(1) << p.cache.page_shift) - 1))) : 0;
+
+    for (int g = part * p.groups_per_part; g < (part + 1) * p.groups_per_part; ++g) {
+        const int head = g * HEADS + lane / LANES;
+        if (head >= heads)
+            break;
+        const unsigned short *from = p.qkv + int64_t(token) * p.token_stride + int64_t(head) * DIM;
+        u32x4_t lo = *reinterpret_cast<const u32x4_t *>(from + low);
+        u32x4_t hi = *reinterpret_cast<const u32x4_t *>(from + high);
+        const bool is_query = head < p.q_heads, is_value = head >= p.q_heads + kv_heads;
+        float x[8], y[8];
+        unpack(lo, x);
+        unpack(hi, y);
+        if (p.q_weight) {
+            float sum = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                sum = fmaf(x[e], x[e], fmaf(y[e], y[e], sum));
+            sum += dpp_move<0xB1>(sum);
+            sum += dpp_move<0x4E>(sum);
+            if (LANES == 8)
+                sum += dpp_move<0x141>(sum);
+            const float inverse = 1.f / sqrtf(sum * (1.f / DIM) + p.epsilon);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                x[e] *= inverse * (is_query ? q_low[e] : k_low[e]);
+                y[e] *= inverse * (is_query ? q_high[e] : k_high[e]);
+            }
+        }
+        if (!is_value) {
+            float a[8], b[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                a[e] = x[e] * c[e] - y[e] * s[e];
+                b[e] = y[e] * c[e] + x[e] * s[e];
+            }
+            // (dims that are not rotated and not normalised pass bit for bit, NaN payloads and infinities too)
+            if (rotates || p.q_weight) {
+                lo = pack(rotates ? a : x);
+                hi = pack(rotates ? b : y);
+            }
+        }
+        if (is_query) {
+            unsigned short *to = p.q_out + int64_t(token) * p.out_stride + int64_t(head) * DIM;
+            *reinterpret_cast<u32x4_t *>(to + low) = lo;
+            *reinterpret_cast<u32x4_t *>(to + high) = hi;
+        } else if (stored) {
+            const int kv = head - p.q_heads - (is_value ? kv_heads : 0);
+            unsigned short *to = (is_value ? p.cache.v : p.cache.k) + row + int64_t(kv) * p.cache.head_stride;
+            *reinterpret_cast<u32x4_t *>(to + low) = lo;
+            *reinterpret_cast<u32x4_t *>(to + high) = hi;
+        }
+    }
+}
+} // namespace
+
+hipError_t launch_qk_norm_rope_append(hipStream_t stream, int tokens, int q_heads, int dim, int rotary, float theta,
+                                      float epsilon, const void *q_weight, const void *k_weight, bool weight_bf16,
+                                      const int32_t *positions, const int64_t *slots, const void *qkv,
+                                      int64_t token_stride, void *q_out, int64_t out_stride, const PagedCache &cache)
+{
+    AppendParams p = {};
+    p.tokens = tokens;
+    p.q_heads = q_heads;
+    p.half = rotary / 2;
+    p.epsilon = epsilon;
+    p.q_weight = q_weight;
+    p.k_weight = k_weight;
+    p.weight_bf16 = weight_bf16;
+    p.positions = positions;
+    p.slots = slots;
+    p.qkv = static_cast<const unsigned short *>(qkv);
+    p.q_out = static_cast<unsigned short *>(q_out);
+    p.token_stride = token_stride;
+    p.out_stride = out_stride;
+    p.cache = cache;
+    for (int i = 0; i < p.half; ++i)
+        p.turns[i] = std::pow(double(theta), -2.0 * i / rotary) / 6.283185307179586476925;
+    const int heads = q_heads + 2 * cache.kv_heads, at_once = 1024 / dim;
+    const int groups = (heads + at_once - 1) / at_once;
+    const int wanted = 2048 / tokens;
+    p.parts = wanted < 1 ? 1 : wanted < groups ? wanted : groups;
+    p.groups_per_part = (groups + p.parts - 1) / p.parts;
+    const int64_t waves = int64_t(tokens) * p.parts;
+    const unsigned blocks = unsigned((waves + APPEND_WAVES - 1) / APPEND_WAVES);
+    if (dim == 128)
+        qk_norm_rope_append_kernel<128><<<blocks, APPEND_WAVES * 64, 0, stream>>>(p);
+    else
+        qk_norm_rope_append_kernel<64><<<blocks, APPEND_WAVES * 64, 0, stream>>>(p);
+    return launch_status();
+}
+} // namespace camblas_hip

@@ -1,0 +1,462 @@
+// One new token of every sequence against its pages: out = softmax(scale q K^T) V over the positions the
+// token sees, grouped query heads, BF16 storage.
+//
+// The kernel is bound by the cache's rows, which are read once: 2 * positions * dim * 2 bytes per
+// key-value head. A wavefront takes 32 positions at a time and runs both products on the matrix cores with
+// the query heads of a group padded to 16 (v_mfma_f32_16x16x32_bf16):
+//   scores  S[position, head] = K[position, :] . Q[head, :]
+//   output  O[dim, head]      = V[position, dim]^T . P[position, head]
+// A lane leaves the first product with head lane % 16 and eight positions, which is the operand layout of
+// the second once the order of its K index is taken to be the order the lane holds. V rows are read with
+// 16 lanes to a row and transposed in registers by byte permutes, so that product w yields the dims
+// (dim / 16) m + w. The running maximum, the sum and the outputs of a head stay in the lanes of that head:
+// the maximum that weights refer to is moved only when a score exceeds it by 2^8, so that the outputs are
+// rarely rescaled; weights are rounded to BF16 for the second product, their sum is kept in FP32.
+//
+// Work is divided by what the sequences hold, not by what the table could hold: all steps of four tiles
+// (sequence, key-value head and 16 query heads, positions) are numbered and every workgroup takes an equal
+// run of them, so lengths may differ by any factor. A workgroup's wavefronts meet in LDS at the end of each
+// (sequence, heads); one that covered it whole writes the output, the others leave a partial (at most two
+// per workgroup) that a second kernel joins in order. Where the workgroups that one (sequence, heads) each
+// would make are enough, there are no partials and one launch.
+#include "common.hpp"
+#include "device.hpp"
+#include "paged_cache.hpp"
+
+namespace camblas_hip
+{
+namespace
+{
+constexpr int WAVES = 4, TILE = 32, HEADS = 16;
+constexpr float LOG2E = 1.4426950408889634f;
+
+struct DecodeParams {
+    int batch, group, head_tiles; // query heads per key-value head, tiles of 16 of them
+    PagedCache cache;
+    PageTable table;
+    Visibility see;
+    float scale; // times log2(e)
+    const unsigned short *q;
+    unsigned short *out;
+    int64_t q_stride, out_stride;
+    float *part_o, *part_m, *part_l; // [2 * workgroups][16][dim], [..][16], [..][16]
+    int2 *joins;                     // per (sequence, heads): first and last workgroup that holds a part of it
+};
+
+// ---- one (sequence, heads): steps first .. last - 1 of it by this workgroup's wavefronts
+
+struct Item {
+    int sequence, kv_head, head0, heads; // first query head and how many of them
+};
+
+template <int DIM> struct Running {
+    static constexpr int DIMS = DIM / 16; // dims a lane holds of a V row
+    f32x4_t acc[DIMS];                    // acc[w][r]: dim DIMS * (4 j + r) + w of head m
+    float top, total;
+};
+
+template <int DIM> struct Tile {
+    bf16x8_t k[2][DIM / 32];
+    unsigned v[8][DIM / 32]; // DIM / 16 values of each of eight positions
+    unsigned mask;           // which of the 32 positions the token sees
+};
+
+template <int DIM>
+__device__ __forceinline__ int fetch_page(const DecodeParams &p, const int32_t *row, int base, int lane)
+{
+    return page_of(p.cache, row, p.table.columns, base + lane % TILE);
+}
+
+template <int DIM>
+__device__ __forceinline__ void load_tile(const DecodeParams &p, int base, int page, int query, size_t head, int lane,
+                                          Tile<DIM> &tile)
+{
+    typedef unsigned row_t __attribute__((ext_vector_type(DIM / 32)));
+    const int m = lane % 16, j = lane / 16;
+    const int position = base + lane % TILE;
+    tile.mask = unsigned(__ballot(page >= 0 && sees(p.see, query, position)));
+    const int known = page < 0 ? 0 : page; // (a masked row is read from some page that exists, and not used)
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const int64_t at = row_offset(p.cache, __shfl(known, 16 * t + m), base + 16 * t + m);
+        const unsigned short *from = p.cache.k + at + head + 8 * j;
+#pragma unroll
+        for (int s = 0; s < DIM / 32; ++s)
+            tile.k[t][s] = *reinterpret_cast<const bf16x8_t *>(from + 32 * s);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const int r = 16 * (e / 4) + 4 * j + e % 4;
+        const int64_t at = row_offset(p.cache, __shfl(known, r), base + r);
+        const row_t got = *reinterpret_cast<const row_t *>(p.cache.v + at + head + (DIM / 16) * m);
+#pragma unroll
+        for (int i = 0; i < DIM / 32; ++i)
+            tile.v[e][i] = got[i];
+    }
+}
+
+template <int DIM>
+__device__ __forceinline__ void attend(const DecodeParams &p, Tile<DIM> &tile, const bf16x8_t (&q)[DIM / 32], int lane,
+                                       Running<DIM> &run)
+{
+    const int j = lane / 16;
+    if (tile.mask == 0)
+        return; // nothing of it is seen (uniform)
+    f32x4_t score[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        score[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < DIM / 32; ++s)
+            score[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(tile.k[t][s], q[s], score[t], 0, 0, 0);
+        score[t] *= p.scale;
+    }
+    if (tile.mask != ~0u) { // (uniform)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const bool seen = (tile.mask >> (16 * (e / 4) + 4 * j + e % 4)) & 1;
+            if (!seen)
+                score[e / 4][e % 4] = -INFINITY;
+            // (a weight of zero times what a hidden row may hold, NaN or infinity, would reach the output)
+#pragma unroll
+            for (int i = 0; i < DIM / 32; ++i)
+                tile.v[e][i] = seen ? tile.v[e][i] : 0u;
+        }
+    }
+    float top = fmaxf(fmaxf(fmaxf(score[0][0], score[0][1]), fmaxf(score[0][2], score[0][3])),
+                      fmaxf(fmaxf(score[1][0], score[1][1]), fmaxf(score[1][2], score[1][3])));
+    if (__any(top > run.top + 8.f)) {
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        top = fmaxf(top, run.top);
+        const float factor = run.top == top ? 1.f : exp2f(run.top - top);
+        run.top = top;
+        run.total *= factor;
+#pragma unroll
+        for (int w = 0; w < DIM / 16; ++w)
+            run.acc[w] *= factor;
+    }
+    const float reference = run.top == -INFINITY ? 0.f : run.top;
+    u32x4_t weights;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            score[t][r] = __builtin_amdgcn_exp2f(score[t][r] - reference);
+            run.total += score[t][r];
+        }
+        weights[2 * t] = pack_bf16x2(score[t][0], score[t][1]);
+        weights[2 * t + 1] = pack_bf16x2(score[t][2], score[t][3]);
+    }
+    const bf16x8_t p_frag = __builtin_bit_cast(bf16x8_t, weights);
+#pragma unroll
+    for (int i = 0; i < DIM / 32; ++i) {
+        u32x4_t even, odd;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            even[c] = __builtin_amdgcn_perm(tile.v[2 * c + 1][i], tile.v[2 * c][i], 0x05040100u);
+            odd[c] = __builtin_amdgcn_perm(tile.v[2 * c + 1][i], tile.v[2 * c][i], 0x07060302u);
+        }
+        run.acc[2 * i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, even), p_frag,
+                                                                  run.acc[2 * i], 0, 0, 0);
+        run.acc[2 * i + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, odd), p_frag,
+                                                                      run.acc[2 * i + 1], 0, 0, 0);
+    }
+}
+
+// slot < 0: this workgroup holds the whole of it and writes the output; otherwise partial `slot`
+template <int DIM>
+__device__ __forceinline__ void work_item(const DecodeParams &p, const Item &item, const TileSpan<TILE> &span, int query,
+                                          int first, int last, int slot)
+{
+    __shared__ float wave_o[WAVES][HEADS][DIM + 4];
+    __shared__ float wave_m[WAVES][HEADS], wave_l[WAVES][HEADS];
+    const int thread = threadIdx.x, lane = thread % 64, wave = thread / 64, m = lane % 16, j = lane / 16;
+    const int32_t *row = p.table.pages + int64_t(item.sequence) * p.table.stride;
+    const size_t head_at = size_t(item.kv_head) * p.cache.head_stride;
+    bf16x8_t q[DIM / 32];
+    {
+        const int head = item.head0 + (m < item.heads ? m : item.heads - 1);
+        const unsigned short *from = p.q + int64_t(item.sequence) * p.q_stride + int64_t(head) * DIM + 8 * j;
+#pragma unroll
+        for (int s = 0; s < DIM / 32; ++s)
+            q[s] = *reinterpret_cast<const bf16x8_t *>(from + 32 * s);
+    }
+    Running<DIM> run;
+    run.top = -INFINITY;
+    run.total = 0.f;
+#pragma unroll
+    for (int w = 0; w < DIM / 16; ++w)
+        run.acc[w] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+
+    const int end = min(last * WAVES, span.tiles);
+    int tile = __builtin_amdgcn_readfirstlane(first * WAVES + wave);
+    if (tile < end) {
+        Tile<DIM> a, b;
+        int base = span.position(tile);
+        int page = fetch_page<DIM>(p, row, base, lane);
+        load_tile<DIM>(p, base, page, query, head_at, lane, a);
+        tile += WAVES;
+        base = span.position(min(tile, span.tiles - 1));
+        page = fetch_page<DIM>(p, row, base, lane);
+        for (;;) {
+            // two tiles a turn, so that both sets of registers have fixed names: the next tile's rows travel
+            // while this one is worked on, and the page numbers of the one after that
+            if (tile < end)
+                load_tile<DIM>(p, base, page, query, head_at, lane, b);
+            base = span.position(min(tile + WAVES, span.tiles - 1));
+            page = fetch_page<DIM>(p, row, base, lane);
+            attend<DIM>(p, a, q, lane, run);
+            if (tile >= end)
+                break;
+            tile += WAVES;
+            if (tile < end)
+                load_tile<DIM>(p, base, page, query, head_at, lane, a);
+            base = span.position(min(tile + WAVES, span.tiles - 1));
+            page = fetch_page<DIM>(p, row, base, lane);
+            attend<DIM>(p, b, q, lane, run);
+            if (tile >= end)
+                break;
+            tile += WAVES;
+        }
+    }
+    run.total += __shfl_xor(run.total, 16);
+    run.total += __shfl_xor(run.total, 32);
+    __syncthreads(); // (the rows below may still be read for the item before)
+    if (j == 0) {
+        wave_m[wave][m] = run.top;
+        wave_l[wave][m] = run.total;
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int w = 0; w < DIM / 16; w += 4)
+            *reinterpret_cast<f32x4_t *>(&wave_o[wave][m][(DIM / 16) * (4 * j + r) + w]) =
+                f32x4_t{run.acc[w][r], run.acc[w + 1][r], run.acc[w + 2][r], run.acc[w + 3][r]};
+    __syncthreads();
+    for (int index = thread; index < item.heads * DIM; index += WAVES * 64) {
+        const int h = index / DIM, d = index % DIM;
+        float best = wave_m[0][h];
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w)
+            best = fmaxf(best, wave_m[w][h]);
+        const float reference = best == -INFINITY ? 0.f : best;
+        float numerator = 0.f, denominator = 0.f;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            const float factor = exp2f(wave_m[w][h] - reference);
+            numerator = fmaf(factor, wave_o[w][h][d], numerator);
+            denominator = fmaf(factor, wave_l[w][h], denominator);
+        }
+        if (slot < 0) {
+            // (no position seen: zero; a sum that is NaN stays NaN)
+            p.out[int64_t(item.sequence) * p.out_stride + int64_t(item.head0 + h) * DIM + d] =
+                float_to_bf16_bits(denominator == 0.f ? 0.f : numerator / denominator);
+        } else {
+            p.part_o[(size_t(slot) * HEADS + h) * DIM + d] = numerator;
+            if (d == 0) {
+                p.part_m[slot * HEADS + h] = best;
+                p.part_l[slot * HEADS + h] = denominator;
+            }
+        }
+    }
+}
+
+__device__ __forceinline__ TileSpan<TILE> span_of(const DecodeParams &p, int sequence, int &query)
+{
+    query = live_positions(p.table, p.cache, sequence) - 1;
+    return TileSpan<TILE>(p.see, query, query);
+}
+
+__device__ __forceinline__ Item item_of(const DecodeParams &p, int sequence, int index)
+{
+    const int kv_head = index / p.head_tiles, tile = index % p.head_tiles;
+    const int first = tile * HEADS;
+    return Item{sequence, kv_head, kv_head * p.group + first, min(HEADS, p.group - first)};
+}
+
+// one workgroup per (heads, sequence)
+template <int DIM> __global__ __launch_bounds__(WAVES * 64, 2) void paged_decode_whole_kernel(DecodeParams p)
+{
+    int query;
+    const TileSpan<TILE> span = span_of(p, blockIdx.y, query);
+    work_item<DIM>(p, item_of(p, blockIdx.y, blockIdx.x), span, query, 0, (span.tiles + WAVES - 1) / WAVES, -1);
+}
+
+// every workgroup an equal run of all steps
+template <int DIM> __global__ __launch_bounds__(WAVES * 64, 2) void paged_decode_shares_kernel(DecodeParams p)
+{
+    constexpr int THREADS = WAVES * 64;
+    __shared__ int64_t wave_total[WAVES];
+    __shared__ int64_t found_start;
+    __shared__ int found_sequence;
+    const int thread = threadIdx.x, lane = thread % 64, wave = thread / 64;
+    const int items = p.cache.kv_heads * p.head_tiles;
+    // steps before each thread's run of sequences
+    const int per = (p.batch + THREADS - 1) / THREADS;
+    const int from = min(thread * per, p.batch), to = min(from + per, p.batch);
+    int64_t mine = 0;
+    for (int b = from; b < to; ++b) {
+        int query;
+        mine += int64_t((span_of(p, b, query).tiles + WAVES - 1) / WAVES) * items;
+    }
+    int64_t before = mine;
+#pragma unroll
+    for (int shift = 1; shift < 64; shift *= 2) {
+        const int64_t other = __shfl_up(before, shift);
+        before += lane >= shift ? other : 0;
+    }
+    if (lane == 63)
+        wave_total[wave] = before;
+    __syncthreads();
+    int64_t all = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+        before += w < wave ? wave_total[w] : 0;
+        all += wave_total[w];
+    }
+    before -= mine;
+    const int64_t workers = min(all, int64_t(gridDim.x)); // each has a step, at least
+    if (int64_t(blockIdx.x) >= workers)
+        return; // (uniform)
+    int64_t step = all * blockIdx.x / workers;
+    const int64_t stop = all * (blockIdx.x + 1) / workers;
+    if (step >= before && step < before + mine) {
+        for (int b = from; b < to; ++b) {
+            int query;
+            const int64_t steps = int64_t((span_of(p, b, query).tiles + WAVES - 1) / WAVES) * items;
+            if (step < before + steps) {
+                found_sequence = b;
+                found_start = before;
+                break;
+            }
+            before += steps;
+        }
+    }
+    __syncthreads();
+    int sequence = __builtin_amdgcn_readfirstlane(found_sequence);
+    int64_t start = found_start;
+    while (step < stop) {
+        int query;
+        const TileSpan<TILE> span = span_of(p, sequence, query);
+        const int steps = (span.tiles + WAVES - 1) / WAVES;
+        while (step < stop && step < start + int64_t(steps) * items) {
+            const int index = int((step - start) / steps);
+            const int64_t begins = start + int64_t(index) * steps;
+            const int first = int(step - begins);
+            const int last = int(min(int64_t(steps), stop - begins));
+            const int slot = first > 0 ? 2 * int(blockIdx.x) : last < steps ? 2 * int(blockIdx.x) + 1 : -1;
+            if (first == 0 && thread == 0) {
+                // the workgroup that holds step s is the last whose run starts at or before it
+                const int64_t ends = ((begins + steps) * workers - 1) / all;
+                p.joins[size_t(sequence) * items + index] = int2{int(blockIdx.x), int(ends)};
+            }
+            work_item<DIM>(p, item_of(p, sequence, index), span, query, first, last, slot);
+            step = begins + last;
+        }
+        start += int64_t(steps) * items;
+        ++sequence;
+    }
+}
+
+// Joins the partials of one (heads, sequence) in the order of its positions; zeros where the sequence holds
+// nothing. One that a single workgroup held is written already.
+template <int DIM> __global__ __launch_bounds__(256) void paged_decode_join_kernel(DecodeParams p)
+{
+    const int items = p.cache.kv_heads * p.head_tiles, sequence = blockIdx.y;
+    const Item item = item_of(p, sequence, blockIdx.x);
+    int query;
+    const bool empty = span_of(p, sequence, query).tiles == 0;
+    const int2 join = empty ? int2{0, 0} : p.joins[size_t(sequence) * items + blockIdx.x];
+    if (!empty && join.x == join.y)
+        return;
+    for (int index = threadIdx.x; index < item.heads * DIM; index += 256) {
+        const int h = index / DIM, d = index % DIM;
+        float best = -INFINITY, numerator = 0.f, denominator = 0.f;
+        if (!empty) {
+            for (int g = join.x; g <= join.y; ++g)
+                best = fmaxf(best, p.part_m[(2 * g + (g == join.x)) * HEADS + h]);
+            const float reference = best == -INFINITY ? 0.f : best;
+            for (int g = join.x; g <= join.y; ++g) {
+                const size_t row = size_t(2 * g + (g == join.x)) * HEADS + h;
+                const float factor = exp2f(p.part_m[row] - reference);
+                numerator = fmaf(factor, p.part_o[row * DIM + d], numerator);
+                denominator = fmaf(factor, p.part_l[row], denominator);
+            }
+        }
+        p.out[int64_t(sequence) * p.out_stride + int64_t(item.head0 + h) * DIM + d] =
+            float_to_bf16_bits(denominator == 0.f ? 0.f : numerator / denominator);
+    }
+}
+} // namespace
+
+// How a call is divided: workgroups that share all steps, or 0 for one workgroup per (heads, sequence).
+static int decode_shares(int64_t items, int64_t positions, int compute_units)
+{
+    const int64_t shares = 2 * int64_t(compute_units);
+    if (positions <= 512 || items >= 4 * shares)
+        return 0;
+    return int(shares);
+}
+
+static int64_t decode_positions(int64_t capacity, const Visibility &see)
+{
+    return see.window > 0 && int64_t(see.window) + see.sinks < capacity ? int64_t(see.window) + see.sinks : capacity;
+}
+
+size_t paged_decode_workspace(int batch, int q_heads, int kv_heads, int dim, int64_t capacity, int window, int sinks,
+                              int compute_units)
+{
+    const int64_t items = int64_t(batch) * kv_heads * ((q_heads / kv_heads + HEADS - 1) / HEADS);
+    const size_t shares = size_t(decode_shares(items, decode_positions(capacity, Visibility{window, sinks}), compute_units));
+    return shares ? 2 * shares * HEADS * (size_t(dim) + 2) * sizeof(float) + size_t(items) * sizeof(int2) : 0;
+}
+
+hipError_t launch_paged_decode(hipStream_t stream, int batch, int q_heads, int dim, const PagedCache &cache,
+                               const PageTable &table, const Visibility &see, float scale, const void *q,
+                               int64_t q_stride, void *out, int64_t out_stride, void *workspace, int compute_units)
+{
+    const int group = q_heads / cache.kv_heads, head_tiles = (group + HEADS - 1) / HEADS;
+    const int items = cache.kv_heads * head_tiles;
+    const int64_t capacity = int64_t(table.columns) << cache.page_shift;
+    const int shares = decode_shares(int64_t(batch) * items, decode_positions(capacity, see), compute_units);
+    DecodeParams p = {};
+    p.batch = batch;
+    p.group = group;
+    p.head_tiles = head_tiles;
+    p.cache = cache;
+    p.table = table;
+    p.see = see;
+    p.scale = scale * LOG2E;
+    p.q = static_cast<const unsigned short *>(q);
+    p.out = static_cast<unsigned short *>(out);
+    p.q_stride = q_stride;
+    p.out_stride = out_stride;
+    if (shares == 0) {
+        const dim3 grid(items, batch);
+        if (dim == 128)
+            paged_decode_whole_kernel<128><<<grid, WAVES * 64, 0, stream>>>(p);
+        else
+            paged_decode_whole_kernel<64><<<grid, WAVES * 64, 0, stream>>>(p);
+        return launch_status();
+    }
+    const size_t rows = 2 * size_t(shares) * HEADS;
+    p.part_o = static_cast<float *>(workspace);
+    p.part_m = p.part_o + rows * dim;
+    p.part_l = p.part_m + rows;
+    p.joins = reinterpret_cast<int2 *>(p.part_l + rows);
+    if (dim == 128)
+        paged_decode_shares_kernel<128><<<shares, WAVES * 64, 0, stream>>>(p);
+    else
+        paged_decode_shares_kernel<64><<<shares, WAVES * 64, 0, stream>>>(p);
+    hipError_t status = launch_status();
+    if (status != hipSuccess)
+        return status;
+    const dim3 grid(items, batch);
+    if (dim == 128)
+        paged_decode_join_kernel<128><<<grid, 256, 0, stream>>>(p);
+    else
+        paged_decode_join_kernel<64><<<grid, 256, 0, stream>>>(p);
+    return launch_status();
+}
+} // namespace camblas_hip

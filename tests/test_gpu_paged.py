@@ -1,0 +1,423 @@
+"""The paged key-value cache on the GPU: append with per-head norm and rotation, decode and prefill attention,
+against their definitions in 64 bits; a run of them together; captured graphs; refusals.
+
+Slots that no sequence holds are filled with NaN and infinities, and table entries behind a sequence's pages
+are out of range: neither may reach an output."""
+
+import ctypes as ct
+import math
+
+import pytest
+import torch
+
+import paged_reference as reference
+from camblas_amd import _kernels, _native
+
+pytestmark = pytest.mark.gpu
+
+
+def queries(seed, tokens, heads, dim, device, scale=1.5):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(tokens, heads, dim, generator=g) * scale).to(torch.bfloat16).to(device)
+
+
+def starts_of(new, device):
+    at = [0]
+    for count in new:
+        at.append(at[-1] + count)
+    return torch.tensor(at, dtype=torch.int32, device=device)
+
+
+def check_decode(device, seed, lengths, *, q_heads, kv_heads, dim, page_size, window=0, sinks=0, scale=None, layout="separate"):
+    k, v, table = reference.paged_case(seed, lengths, page_size=page_size, kv_heads=kv_heads, dim=dim, device=device, layout=layout)
+    q = queries(seed + 1, len(lengths), q_heads, dim, device)
+    held = torch.tensor(lengths, dtype=torch.int32, device=device)
+    got = _kernels.paged_decode_attention(q, k, v, table, held, window=window, sinks=sinks, scale=scale)
+    want, allowed = reference.attention_rows(q, k, v, table, lengths, [1] * len(lengths), window=window, sinks=sinks, scale=scale)
+    assert reference.within(got, want, allowed)
+    return got
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("page_size", [1, 16, 64])
+@pytest.mark.parametrize("q_heads,kv_heads", [(8, 1), (6, 3), (4, 4), (20, 1), (66, 2)])
+def test_decode_lengths_heads_and_pages(device, dim, page_size, q_heads, kv_heads):
+    check_decode(device, 100, [1, 31, 32, 33, 0, 127, 128, 129, 300, 5], q_heads=q_heads, kv_heads=kv_heads, dim=dim, page_size=page_size)
+
+
+@pytest.mark.parametrize("page_size", [2, 4, 8, 32, 128, 1024])
+def test_decode_page_sizes(device, page_size):
+    check_decode(device, 150, [700, 1, 65, 511], q_heads=8, kv_heads=2, dim=128, page_size=page_size)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (7, 3), (32, 0), (33, 64), (100, 4), (128, 33), (1000, 2000), (5000, 4)])
+def test_decode_windows_and_first_tokens(device, dim, window, sinks):
+    check_decode(device, 200, [1, 2, 31, 64, 65, 100, 101, 160, 777, 0], q_heads=10, kv_heads=2, dim=dim, page_size=16, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("lengths", [[4000], [1, 3000, 1, 1, 2500, 0, 0, 700], [513] * 20, [0, 0, 2000], [1] * 300 + [1500]])
+def test_decode_divided_over_workgroups(device, lengths):
+    check_decode(device, 300, lengths, q_heads=8, kv_heads=2, dim=128, page_size=16)
+
+
+@pytest.mark.parametrize("layout", ["together", "heads first"])
+def test_decode_layouts_of_the_cache(device, layout):
+    check_decode(device, 400, [5, 200, 1030], q_heads=9, kv_heads=3, dim=64, page_size=16, layout=layout)
+
+
+def test_decode_strided_queries_outputs_and_table(device):
+    lengths = [40, 3, 700]
+    k, v, table = reference.paged_case(500, lengths, page_size=16, kv_heads=2, dim=128, device=device)
+    qkv = queries(501, 3, 12, 128, device)
+    wide = torch.full((3, table.shape[1] + 5), -7, dtype=torch.int32, device=device)
+    wide[:, : table.shape[1]] = table
+    out = torch.full((3, 16, 128), 9.0, dtype=torch.bfloat16, device=device)
+    held = torch.tensor(lengths, dtype=torch.int32, device=device)
+    _kernels.paged_decode_attention(qkv[:, :8], k, v, wide[:, : table.shape[1]], held, out=out[:, 4:12])
+    plain = _kernels.paged_decode_attention(qkv[:, :8].contiguous(), k, v, table, held)
+    assert torch.equal(out[:, 4:12], plain)
+    assert (out[:, :4] == 9).all() and (out[:, 12:] == 9).all()
+
+
+def test_decode_pages_that_do_not_exist_hold_nothing(device):
+    lengths = [200, 64]
+    k, v, table = reference.paged_case(600, lengths, page_size=16, kv_heads=1, dim=128, device=device)
+    table[0, 3], table[0, 7], table[0, 12] = -1, k.shape[0], -2**31
+    table[1, :] = 2**30  # a sequence none of whose pages exists
+    q = queries(601, 2, 8, 128, device)
+    got = _kernels.paged_decode_attention(q, k, v, table, torch.tensor([200, 64], dtype=torch.int32, device=device))
+    want, allowed = reference.attention_rows(q, k, v, table, lengths, [1, 1])
+    assert reference.within(got, want, allowed) and not got[1].any()
+
+
+def test_decode_lengths_outside_the_table(device):
+    k, v, table = reference.paged_case(650, [64, 64, 64], page_size=16, kv_heads=1, dim=64, device=device, poison=False)
+    table = table[:, :4].contiguous()
+    q = queries(651, 3, 4, 64, device)
+    got = _kernels.paged_decode_attention(q, k, v, table, torch.tensor([2**31 - 1, -5, 65], dtype=torch.int32, device=device))
+    want, allowed = reference.attention_rows(q, k, v, table, [64, 0, 64], [1, 1, 1])
+    assert reference.within(got, want, allowed)
+
+
+def test_decode_values_that_are_not_numbers_where_they_are_seen(device):
+    lengths = [100, 100, 100]
+    k, v, table = reference.paged_case(700, lengths, page_size=16, kv_heads=1, dim=128, device=device)
+    rows = [(int(table[b, 40 // 16]), 40 % 16) for b in range(3)]
+    v[rows[0]][0, 5] = math.nan
+    v[rows[1]][0, 6] = math.inf
+    k[rows[2]][0, 7] = math.nan
+    q = queries(701, 3, 8, 128, device)
+    got = _kernels.paged_decode_attention(q, k, v, table, torch.tensor(lengths, dtype=torch.int32, device=device))
+    assert torch.isnan(got[0, :, 5]).all() and torch.isinf(got[1, :, 6]).all() and torch.isnan(got[2]).all()
+    assert torch.isnan(got[0]).sum() == 8 and not torch.isnan(got[1]).any() and torch.isinf(got[1]).sum() == 8
+
+
+def test_decode_far_scores_and_extreme_scales(device):
+    # scores of +-700: weights underflow, the maximum moves by hundreds between tiles
+    lengths = [640]
+    k, v, table = reference.paged_case(750, lengths, page_size=16, kv_heads=1, dim=64, device=device)
+    q = queries(751, 1, 8, 64, device, scale=30.0)
+    got = _kernels.paged_decode_attention(q, k, v, table, torch.tensor(lengths, dtype=torch.int32, device=device), scale=1.0)
+    want, allowed = reference.attention_rows(q, k, v, table, lengths, [1], scale=1.0)
+    assert reference.within(got, want, allowed)
+
+
+def check_prefill(device, seed, new, past, *, q_heads, kv_heads, dim, page_size, window=0, sinks=0, layout="separate"):
+    lengths = [n + p for n, p in zip(new, past)]
+    k, v, table = reference.paged_case(seed, lengths, page_size=page_size, kv_heads=kv_heads, dim=dim, device=device, layout=layout)
+    q = queries(seed + 1, sum(new) + 3, q_heads, dim, device)
+    out = torch.full(q.shape, 5.0, dtype=torch.bfloat16, device=device)
+    _kernels.paged_prefill_attention(q, k, v, table, torch.tensor(lengths, dtype=torch.int32, device=device),
+                                     starts_of(new, device), window=window, sinks=sinks, out=out)
+    want, allowed = reference.attention_rows(q, k, v, table, lengths, new, window=window, sinks=sinks)
+    assert reference.within(out[: sum(new)], want, allowed)
+    assert (out[sum(new):] == 5).all()  # rows behind the last sequence
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("q_heads,kv_heads", [(8, 1), (4, 4), (6, 2), (7, 1), (20, 1)])
+def test_prefill_ragged(device, dim, q_heads, kv_heads):
+    check_prefill(device, 1000, [1, 17, 0, 64, 65, 3], [0, 40, 9, 0, 63, 200], q_heads=q_heads, kv_heads=kv_heads, dim=dim, page_size=16)
+
+
+@pytest.mark.parametrize("page_size", [1, 8, 64, 256])
+def test_prefill_page_sizes(device, page_size):
+    check_prefill(device, 1100, [70, 5, 128], [0, 333, 1], q_heads=4, kv_heads=2, dim=128, page_size=page_size)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("window,sinks", [(1, 0), (1, 2), (16, 4), (64, 0), (65, 70), (100, 1), (1000, 8)])
+def test_prefill_windows_and_first_tokens(device, dim, window, sinks):
+    check_prefill(device, 1200, [150, 33, 1], [0, 190, 64], q_heads=6, kv_heads=2, dim=dim, page_size=16, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("layout", ["together", "heads first"])
+def test_prefill_layouts_of_the_cache(device, layout):
+    check_prefill(device, 1300, [40, 100], [10, 0], q_heads=4, kv_heads=2, dim=128, page_size=16, layout=layout)
+
+
+def test_prefill_more_queries_than_positions(device):
+    # 10 new tokens, 4 positions in the cache: the first six see nothing
+    k, v, table = reference.paged_case(1400, [4, 20], page_size=4, kv_heads=1, dim=64, device=device)
+    q = queries(1401, 30, 4, 64, device)
+    new, lengths = [10, 20], [4, 20]
+    got = _kernels.paged_prefill_attention(q, k, v, table, torch.tensor(lengths, dtype=torch.int32, device=device), starts_of(new, device))
+    want, allowed = reference.attention_rows(q, k, v, table, lengths, new)
+    assert reference.within(got, want, allowed) and not got[:6].any()
+
+
+def test_prefill_pages_that_do_not_exist_hold_nothing(device):
+    new, lengths = [30, 50], [200, 50]
+    k, v, table = reference.paged_case(1500, lengths, page_size=16, kv_heads=2, dim=128, device=device)
+    table[0, 2], table[0, 11], table[1, :] = -3, k.shape[0], 2**31 - 1
+    q = queries(1501, 80, 8, 128, device)
+    got = _kernels.paged_prefill_attention(q, k, v, table, torch.tensor(lengths, dtype=torch.int32, device=device), starts_of(new, device))
+    want, allowed = reference.attention_rows(q, k, v, table, lengths, new)
+    assert reference.within(got, want, allowed) and not got[30:].any()
+
+
+def test_prefill_one_token_each_equals_decode_within_rounding(device):
+    lengths = [1, 70, 1030, 257]
+    k, v, table = reference.paged_case(1600, lengths, page_size=16, kv_heads=2, dim=128, device=device)
+    q = queries(1601, 4, 16, 128, device)
+    held = torch.tensor(lengths, dtype=torch.int32, device=device)
+    a = _kernels.paged_decode_attention(q, k, v, table, held)
+    b = _kernels.paged_prefill_attention(q, k, v, table, held, starts_of([1] * 4, device))
+    want, allowed = reference.attention_rows(q, k, v, table, lengths, [1] * 4)
+    assert reference.within(a, want, allowed) and reference.within(b, want, allowed)
+
+
+APPEND_CASES = [
+    # tokens, q_heads, kv_heads, dim, rotary, norm, page_size
+    (1, 64, 8, 128, 128, torch.bfloat16, 16), (7, 6, 2, 64, 64, torch.float32, 1), (33, 5, 1, 128, 64, None, 4),
+    (130, 3, 3, 64, 16, torch.bfloat16, 64), (65, 8, 8, 128, 0, torch.float32, 16), (3000, 4, 1, 64, 32, torch.bfloat16, 16),
+    (2, 1, 1, 128, 112, None, 32)]
+
+
+@pytest.mark.parametrize("tokens,q_heads,kv_heads,dim,rotary,norm,page_size", APPEND_CASES)
+def test_append(device, tokens, q_heads, kv_heads, dim, rotary, norm, page_size):
+    g = torch.Generator().manual_seed(2000 + tokens)
+    wide = torch.randn(tokens, q_heads + 2 * kv_heads + 1, dim, generator=g).to(torch.bfloat16)
+    wide[0, 0] *= 1e-4  # a head whose mean square is of the size of epsilon
+    wide = wide.to(device)
+    qkv = wide[:, : q_heads + 2 * kv_heads]
+    positions = torch.randint(0, 2**31 - 1, (tokens,), generator=g, dtype=torch.int64).to(torch.int32)
+    positions[0] = 0
+    pages = -(-tokens // page_size) + 2
+    slots = torch.randperm(pages * page_size, generator=g)[:tokens]
+    slots[tokens // 3 + 1::5] = -1
+    if tokens > 2:
+        slots[-1] = pages * page_size  # the first behind the cache
+    weights = [None, None] if norm is None else [(1 + 0.3 * torch.randn(dim, generator=g)).to(norm).to(device) for _ in range(2)]
+    before = torch.randn(2, pages, page_size, kv_heads, dim, generator=g).to(torch.bfloat16).to(device)
+    k, v = before[0].clone(), before[1].clone()
+    got = _kernels.qk_norm_rope_append(qkv, positions.to(device), slots.to(device), k, v, q_heads=q_heads, kv_heads=kv_heads,
+                                       q_weight=weights[0], k_weight=weights[1], epsilon=1e-6, theta=10000.0, rotary_dim=rotary)
+    q_want, k_want, q_off, k_off = reference.append(qkv, positions, q_heads=q_heads, kv_heads=kv_heads, q_weight=weights[0],
+                                                    k_weight=weights[1], epsilon=1e-6, theta=10000.0, rotary=rotary)
+    assert reference.within(got, q_want, q_off)
+    kept = (slots >= 0) & (slots < pages * page_size)
+    where = slots[kept].to(device)
+    assert reference.within(k.view(-1, kv_heads, dim)[where], k_want[kept], k_off[kept])
+    assert torch.equal(v.view(-1, kv_heads, dim)[where], qkv[:, q_heads + kv_heads:][kept.to(device)])
+    others = torch.ones(pages * page_size, dtype=torch.bool, device=device)
+    others[where] = False
+    for cache, old in ((k, before[0]), (v, before[1])):
+        assert torch.equal(cache.view(-1, kv_heads, dim)[others], old.view(-1, kv_heads, dim)[others])
+
+
+def test_append_in_place_and_into_views_of_one_cache(device):
+    tokens, q_heads, kv_heads, dim = 50, 12, 3, 128
+    qkv = queries(2100, tokens, q_heads + 2 * kv_heads, dim, device)
+    weight = torch.rand(dim, device=device) + 0.5
+    positions = torch.arange(tokens, dtype=torch.int32, device=device)
+    slots = torch.arange(tokens, device=device) * 2
+    options = dict(q_heads=q_heads, kv_heads=kv_heads, q_weight=weight, k_weight=weight, rotary_dim=64)
+    k, v = (torch.zeros(8, 16, kv_heads, dim, dtype=torch.bfloat16, device=device) for _ in range(2))
+    apart = _kernels.qk_norm_rope_append(qkv, positions, slots, k, v, **options)
+    both = torch.zeros(8, 2, kv_heads, 16, dim, dtype=torch.bfloat16, device=device)
+    k2, v2 = both[:, 0].transpose(1, 2), both[:, 1].transpose(1, 2)
+    copy = qkv.clone()
+    _kernels.qk_norm_rope_append(copy, positions, slots, k2, v2, out=copy[:, :q_heads], **options)
+    assert torch.equal(copy[:, :q_heads], apart) and torch.equal(copy[:, q_heads:], qkv[:, q_heads:])
+    assert torch.equal(k2, k) and torch.equal(v2, v)
+
+
+def test_a_sequence_from_prompt_to_decode_steps(device):
+    """A prompt in two ragged chunks, then single tokens, through append and attention; every attention against
+    the definition on what the caches hold."""
+    q_heads, kv_heads, dim, page_size = 8, 2, 128, 16
+    g = torch.Generator().manual_seed(2200)
+    table = torch.randperm(40, generator=g).to(torch.int32).view(2, 20).to(device)
+    k, v = (torch.full((40, page_size, kv_heads, dim), math.nan, dtype=torch.bfloat16, device=device) for _ in range(2))
+    weight = (torch.rand(dim, generator=g) + 0.5).to(device)
+    held = [0, 0]
+    for step, new in enumerate([[100, 37], [60, 0], [1, 90], [1, 1], [1, 1]]):
+        tokens = sum(new)
+        qkv = queries(2201 + step, tokens, q_heads + 2 * kv_heads, dim, device)
+        position = torch.cat([torch.arange(held[b], held[b] + new[b]) for b in range(2)]).to(torch.int32).to(device)
+        sequence = torch.tensor([0] * new[0] + [1] * new[1], device=device)
+        slots = table[sequence, (position // page_size).long()].long() * page_size + position % page_size
+        q = _kernels.qk_norm_rope_append(qkv, position, slots, k, v, q_heads=q_heads, kv_heads=kv_heads, q_weight=weight, k_weight=weight)
+        held = [held[b] + new[b] for b in range(2)]
+        lengths = torch.tensor(held, dtype=torch.int32, device=device)
+        if new == [1, 1]:
+            got = _kernels.paged_decode_attention(q, k, v, table, lengths, window=64, sinks=4)
+        else:
+            got = _kernels.paged_prefill_attention(q, k, v, table, lengths, starts_of(new, device), window=64, sinks=4)
+        want, allowed = reference.attention_rows(q, k, v, table, held, new, window=64, sinks=4)
+        assert reference.within(got, want, allowed), step
+
+
+def test_captured_steps_replay_with_other_lengths(device):
+    """Append and both attentions in two graphs on one stream; lengths, slots and inputs change between replays."""
+    q_heads, kv_heads, dim, page_size, batch = 8, 1, 128, 16, 3
+    k, v, table = reference.paged_case(2300, [1400, 900, 640], page_size=page_size, kv_heads=kv_heads, dim=dim, device=device)
+    table = table[:, :88].contiguous()
+    stream = torch.cuda.Stream()
+    lengths = torch.tensor([1, 1, 1], dtype=torch.int32, device=device)
+    qkv = queries(2301, batch, q_heads + 2 * kv_heads, dim, device)
+    new = torch.tensor([0, 1, 2, 3], dtype=torch.int32, device=device)
+
+    def step():
+        position = lengths - 1
+        slots = table.gather(1, (position // page_size).long()[:, None])[:, 0].long() * page_size + position % page_size
+        q = _kernels.qk_norm_rope_append(qkv, position, slots, k, v, q_heads=q_heads, kv_heads=kv_heads)
+        return q, _kernels.paged_decode_attention(q, k, v, table, lengths), _kernels.paged_prefill_attention(q, k, v, table, lengths, new)
+
+    graphs = []
+    with torch.cuda.stream(stream):
+        step()
+        torch.cuda.synchronize()
+        for _ in range(2):
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                held = step()
+            graphs.append((graph, held))
+    torch.cuda.synchronize()
+    for turn, held in enumerate([[3, 900, 17], [1400, 1, 640], [33, 511, 512]]):
+        lengths.copy_(torch.tensor(held, dtype=torch.int32))
+        qkv.copy_(queries(2310 + turn, batch, q_heads + 2 * kv_heads, dim, device))
+        eager = [t.clone() for t in step()]
+        torch.cuda.synchronize()
+        for graph, outputs in graphs:
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(outputs, eager)), turn
+        want, allowed = reference.attention_rows(eager[0], k, v, table, held, [1, 1, 1])
+        assert reference.within(eager[1], want, allowed) and reference.within(eager[2], want, allowed)
+
+
+def test_results_repeat_bit_for_bit_on_two_streams(device):
+    lengths = [5000, 3, 700, 2048]
+    k, v, table = reference.paged_case(2400, lengths, page_size=16, kv_heads=2, dim=64, device=device)
+    q = queries(2401, 4, 14, 64, device)
+    held = torch.tensor(lengths, dtype=torch.int32, device=device)
+    first = _kernels.paged_decode_attention(q, k, v, table, held)
+    torch.cuda.synchronize()
+    streams, outs = [torch.cuda.Stream() for _ in range(2)], []
+    for _ in range(3):
+        for stream in streams:
+            with torch.cuda.stream(stream):
+                outs.append(_kernels.paged_decode_attention(q, k, v, table, held))
+    torch.cuda.synchronize()
+    assert all(torch.equal(first, other) for other in outs)
+
+
+def test_empty_batches(device):
+    k, v, table = reference.paged_case(2500, [20], page_size=16, kv_heads=1, dim=64, device=device)
+    none = torch.zeros(0, dtype=torch.int32, device=device)
+    q = queries(2501, 0, 4, 64, device)
+    assert _kernels.paged_decode_attention(q, k, v, table[:0], none).shape == (0, 4, 64)
+    assert _kernels.paged_prefill_attention(q, k, v, table[:0], none, torch.zeros(1, dtype=torch.int32, device=device)).shape == (0, 4, 64)
+    assert _kernels.qk_norm_rope_append(queries(2502, 0, 6, 64, device), none, none.long(), k, v, q_heads=4, kv_heads=1).shape == (0, 4, 64)
+    # sequences, but a table without columns: nothing is held
+    q = queries(2503, 2, 4, 64, device)
+    held = torch.tensor([7, 1], dtype=torch.int32, device=device)
+    assert not _kernels.paged_decode_attention(q, k, v, table[:1, :0].expand(2, 0).contiguous(), held).any()
+
+
+def refused(call, *arguments, **options):
+    with pytest.raises((RuntimeError, ct.ArgumentError, TypeError)):
+        call(*arguments, **options)
+
+
+def test_refusals(device):
+    lengths = [40, 3]
+    k, v, table = reference.paged_case(2600, lengths, page_size=16, kv_heads=2, dim=128, device=device)
+    q = queries(2601, 2, 8, 128, device)
+    held = torch.tensor(lengths, dtype=torch.int32, device=device)
+    decode = _kernels.paged_decode_attention
+    decode(q, k, v, table, held)
+    refused(decode, q.float(), k, v, table, held)
+    refused(decode, q.cpu(), k, v, table, held)
+    refused(decode, q[:, :7], k, v, table, held)                      # heads not a multiple of the cache's
+    refused(decode, q[:, :, :64], k, v, table, held)                  # another head size
+    refused(decode, q[:1], k, v, table, held)                         # one query, two sequences
+    refused(decode, q, k, v[:-1], table, held)
+    refused(decode, q, k, k, table, held)                             # keys and values in one place
+    refused(decode, q, k.float(), v.float(), table, held)
+    refused(decode, q, k[:, :12], v[:, :12], table, held)             # pages of twelve
+    refused(decode, q, k, v, table.long(), held)
+    refused(decode, q, k, v, table.t().contiguous().t(), held)        # columns apart
+    refused(decode, q, k, v, table, held.long())
+    refused(decode, q, k, v, table, held[:1])
+    for scale in (0.0, -1.0, math.nan, math.inf):
+        refused(decode, q, k, v, table, held, scale=scale)
+    refused(decode, q, k, v, table, held, window=-1)
+    refused(decode, q, k, v, table, held, sinks=-1)
+    refused(decode, q, k, v, table, held, out=q)
+    refused(decode, q.clone().requires_grad_(), k, v, table, held)
+    starts = torch.tensor([0, 1, 2], dtype=torch.int32, device=device)
+    prefill = _kernels.paged_prefill_attention
+    prefill(q, k, v, table, held, starts)
+    refused(prefill, q, k, v, table, held, starts[:2])
+    refused(prefill, q, k, v, table, held, starts.long())
+    refused(prefill, q, k, v, table, held, starts, window=-2)
+    refused(prefill, q, k, v, table, held, starts, out=q)
+    qkv = queries(2602, 2, 12, 128, device)
+    position, slots = held - 1, torch.tensor([0, 1], device=device)
+    append = _kernels.qk_norm_rope_append
+    options = dict(q_heads=8, kv_heads=2)
+    weight = torch.ones(128, device=device)
+    append(qkv, position, slots, k, v, **options)
+    refused(append, qkv, position, slots, k, v, q_heads=7, kv_heads=2)
+    refused(append, qkv, position, slots, k, v, q_heads=10, kv_heads=1)
+    refused(append, qkv, position.long(), slots, k, v, **options)
+    refused(append, qkv, position, slots.int(), k, v, **options)
+    refused(append, qkv, position, slots, k, v, q_weight=weight, **options)
+    refused(append, qkv, position, slots, k, v, q_weight=weight, k_weight=weight.bfloat16(), **options)
+    refused(append, qkv, position, slots, k, v, q_weight=weight[:64], k_weight=weight[:64], **options)
+    for rotary in (8, 136, -16, 120):
+        refused(append, qkv, position, slots, k, v, rotary_dim=rotary, **options)
+    for theta in (0.0, -5.0, math.nan):
+        refused(append, qkv, position, slots, k, v, theta=theta, **options)
+    refused(append, qkv, position, slots, k, v, epsilon=-1.0, **options)
+    refused(append, qkv, position, slots, k, v, out=torch.empty(2, 7, 128, dtype=torch.bfloat16, device=device), **options)
+
+
+def test_the_c_entry_refuses_a_small_or_missing_workspace(device):
+    lengths = [2000]
+    k, v, table = reference.paged_case(2700, lengths, page_size=16, kv_heads=1, dim=64, device=device)
+    q = queries(2701, 1, 4, 64, device)
+    out = torch.zeros_like(q)
+    held = torch.tensor(lengths, dtype=torch.int32, device=device)
+    native = _native.context(device)
+    cache = _kernels._paged_cache(k, v, q)
+    columns = table.shape[1]
+    size = _native.library().camblas_cuda_paged_decode_workspace_size(native.handle, 1, 4, ct.byref(cache), columns, 0, 0)
+    assert size > 0
+    room = torch.empty(size + 16, dtype=torch.uint8, device=device)
+
+    def call(address, count):
+        native.call("paged_decode_attention", 1, 4, ct.byref(cache), table.data_ptr(), columns, columns, held.data_ptr(), 0, 0, 0.125,
+                    q.data_ptr(), 256, address, count, out.data_ptr(), 256)
+
+    for address, count in ((None, size), (room.data_ptr(), size - 1), (room.data_ptr() + 4, size)):
+        with pytest.raises(RuntimeError, match="workspace"):
+            call(address, count)
+    assert not out.any()
+    call(room.data_ptr(), size)
+    want, allowed = reference.attention_rows(q, k, v, table, lengths, [1])
+    assert reference.within(out, want, allowed)
