@@ -123,7 +123,8 @@ def build_probes():
     return target
 
 
-BINDING_SOURCES = ("tensor_binding.cpp", "binding_dense.cpp", "binding_fusion.cpp", "binding_quantized.cpp")
+BINDING_SOURCES = ("tensor_binding.cpp", "binding_dense.cpp", "binding_fusion.cpp", "binding_quantized.cpp",
+                   "binding_paged.cpp")
 
 
 def build_tensor_binding(jobs=4):

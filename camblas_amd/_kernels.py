@@ -782,36 +782,15 @@ def rope_append_attention(qkv, positions, k_cache, v_cache, *, q_heads, kv_heads
     return out
 
 
-def _paged_cache(k_cache, v_cache, reference):
-    """The C description of BF16 pages [pages, page_size, kv_heads, dim] (any strides in multiples of eight
-    with contiguous heads, e.g. views of one [pages, 2, page_size, kv_heads, dim] tensor)."""
-    _require(k_cache.dtype == v_cache.dtype == torch.bfloat16 and k_cache.dim() == 4
-             and k_cache.shape == v_cache.shape and k_cache.stride() == v_cache.stride()
-             and k_cache.device == v_cache.device == reference.device,
-             "a paged cache is two BF16 tensors [pages, page_size, kv_heads, dim] of one layout on the operands' device")
-    pages, page_size, kv_heads, dim = k_cache.shape
-    page_stride, slot_stride, head_stride, unit = k_cache.stride()
-    _require(dim in (64, 128) and unit == 1 and pages > 0 and kv_heads > 0, "paged heads must hold 64 or 128 contiguous values")
-    return _native.PagedCache(k_cache.data_ptr(), v_cache.data_ptr(), page_stride, slot_stride, head_stride, pages,
-                              page_size, kv_heads, dim)
+def _tensor_binding():
+    module = tensor_module()
+    if module is None or not hasattr(module, "paged_decode_attention"):
+        raise RuntimeError("the paged cache requires the tensor binding (python camblas_amd/_build.py)")
+    return module
 
 
-def _paged_rows(tensor, name, tokens, heads, dim, device):
-    """The token stride of BF16 rows [tokens, heads, dim] whose heads lie next to each other."""
-    _require(tensor.dtype == torch.bfloat16 and tuple(tensor.shape) == (tokens, heads, dim) and tensor.device == device
-             and tensor.stride(2) == 1 and (heads == 1 or tensor.stride(1) == dim),
-             f"{name} must be BF16 [{tokens}, {heads}, {dim}] with dense heads on the operands' device")
-    return tensor.stride(0)
-
-
-def _integers(tensor, name, dtype, shape, device):
-    _require(tensor.dtype == dtype and tuple(tensor.shape) == shape and tensor.is_contiguous() and tensor.device == device,
-             f"{name} must be contiguous {dtype} {list(shape)} on the operands' device")
-
-
-def _inference_only(*tensors):
-    _require(not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in tensors),
-             "the paged cache's operators support inference only")
+# The paged cache's operators go through the tensor binding: a decode step's kernels take a few microseconds,
+# less than checking and passing a dozen arguments through ctypes (16 against 6 us a call).
 
 
 def qk_norm_rope_append(qkv, positions, slots, k_cache, v_cache, *, q_heads, kv_heads, q_weight=None, k_weight=None,
@@ -823,83 +802,32 @@ def qk_norm_rope_append(qkv, positions, slots, k_cache, v_cache, *, q_heads, kv_
     are given, and rotated by halves over their first rotary_dim dims (default: all; a multiple of 16) by
     positions (int32 [tokens]); FP32 arithmetic, angles in FP64, one rounding. slots (int64 [tokens]) says
     where keys and values go: page * page_size + place; one outside the cache (-1 for padding rows) writes
-    nothing. k_cache and v_cache are [pages, page_size, kv_heads, dim]. `out` may be qkv[:, :q_heads].
+    nothing. k_cache and v_cache are BF16 [pages, page_size, kv_heads, dim] of one layout, dim 64 or 128, page_size
+    a power of two, strides in multiples of eight with contiguous heads (e.g. views of one [pages, 2, page_size,
+    kv_heads, dim] tensor). `out` may be qkv[:, :q_heads].
     """
-    _require(qkv.dim() == 3 and qkv.is_cuda and q_heads >= 1 and kv_heads >= 1, "qkv must be BF16 [tokens, Hq + 2 Hkv, dim] on a GPU")
-    _inference_only(qkv, q_weight, k_weight, k_cache, v_cache)
-    tokens, _, dim = qkv.shape
-    device = qkv.device
-    cache = _paged_cache(k_cache, v_cache, qkv)
-    _require(cache.kv_heads == kv_heads and cache.dim == dim, "the cache's heads differ from the activation's")
-    token_stride = _paged_rows(qkv, "qkv", tokens, q_heads + 2 * kv_heads, dim, device)
-    _integers(positions, "positions", torch.int32, (tokens,), device)
-    _integers(slots, "slots", torch.int64, (tokens,), device)
-    _require((q_weight is None) == (k_weight is None), "query and key norm weights come together")
-    if q_weight is not None:
-        _require(q_weight.dtype == k_weight.dtype and q_weight.dtype in (torch.float32, torch.bfloat16)
-                 and tuple(q_weight.shape) == tuple(k_weight.shape) == (dim,) and q_weight.is_contiguous()
-                 and k_weight.is_contiguous() and q_weight.device == k_weight.device == device,
-                 "norm weights must be contiguous FP32 or BF16 [dim] on the operands' device")
-    if out is None:
-        out = torch.empty((tokens, q_heads, dim), dtype=torch.bfloat16, device=device)
-    out_stride = _paged_rows(out, "out", tokens, q_heads, dim, device)
-    _native.context(device).call(
-        "qk_norm_rope_append", tokens, q_heads, dim if rotary_dim is None else rotary_dim, theta,
-        0 if q_weight is None else _DTYPE_CODE[q_weight.dtype], epsilon, _pointer(q_weight), _pointer(k_weight),
-        positions.data_ptr(), slots.data_ptr(), qkv.data_ptr(), token_stride, out.data_ptr(), out_stride, ct.byref(cache))
-    return out
-
-
-def _paged_attention_operands(q, k_cache, v_cache, page_table, lengths, scale, out):
-    _require(q.dim() == 3 and q.is_cuda, "q must be BF16 [tokens, heads, dim] on a GPU")
-    _inference_only(q, k_cache, v_cache)
-    cache = _paged_cache(k_cache, v_cache, q)
-    tokens, q_heads, dim = q.shape
-    _require(dim == cache.dim, "the cache's heads differ from the queries'")
-    q_stride = _paged_rows(q, "q", tokens, q_heads, dim, q.device)
-    _require(page_table.dtype == torch.int32 and page_table.dim() == 2 and page_table.device == q.device
-             and (page_table.shape[1] < 2 or page_table.stride(1) == 1), "page_table must be int32 [batch, columns] with dense rows")
-    _integers(lengths, "lengths", torch.int32, (page_table.shape[0],), q.device)
-    if out is None:
-        out = torch.empty((tokens, q_heads, dim), dtype=torch.bfloat16, device=q.device)
-    out_stride = _paged_rows(out, "out", tokens, q_heads, dim, q.device)
-    return cache, q_stride, out, out_stride, dim**-0.5 if scale is None else scale
+    return _tensor_binding().qk_norm_rope_append(
+        qkv, positions, slots, k_cache, v_cache, q_heads=q_heads, kv_heads=kv_heads, q_weight=q_weight, k_weight=k_weight,
+        epsilon=epsilon, theta=theta, rotary_dim=rotary_dim, out=out)
 
 
 def paged_decode_attention(q, k_cache, v_cache, page_table, lengths, *, scale=None, window=0, sinks=0, out=None):
     """Attention of one new token per sequence, q [batch, q_heads, dim], over pages [pages, page_size,
-    kv_heads, dim] found through page_table (int32 [batch, columns]); lengths (int32 [batch]) counts the
-    positions of each sequence, the new token's among them. window > 0: only the last `window` positions and
-    the first `sinks` are seen. BF16 [batch, q_heads, dim]; zeros where nothing is seen."""
-    cache, q_stride, out, out_stride, scale = _paged_attention_operands(q, k_cache, v_cache, page_table, lengths, scale, out)
-    batch, q_heads, _ = q.shape
-    _require(page_table.shape[0] == batch, "one query, one table row and one length per sequence")
-    native = _native.context(q.device)
-    columns = page_table.shape[1]
-    described = ct.byref(cache)
-    size = _native.library().camblas_cuda_paged_decode_workspace_size(native.handle, batch, q_heads, described, columns, window, sinks)
-    workspace = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
-    native.call("paged_decode_attention", batch, q_heads, described, page_table.data_ptr(), page_table.stride(0), columns,
-                lengths.data_ptr(), window, sinks, scale, q.data_ptr(), q_stride,
-                workspace.data_ptr() if size else None, size, out.data_ptr(), out_stride)
-    return out
+    kv_heads, dim] found through page_table (int32 [batch, columns]; entries that are no page hold nothing); lengths
+    (int32 [batch]) counts the positions of each sequence, the new token's among them. window > 0: only the last
+    `window` positions and the first `sinks` are seen. BF16 [batch, q_heads, dim]; zeros where nothing is seen."""
+    return _tensor_binding().paged_decode_attention(q, k_cache, v_cache, page_table, lengths, scale=scale, window=window,
+                                                    sinks=sinks, out=out)
 
 
 def paged_prefill_attention(q, k_cache, v_cache, page_table, lengths, query_starts, *, scale=None, window=0, sinks=0, out=None):
     """Causal attention of the new tokens of ragged sequences, q [tokens, q_heads, dim], over the pages that
     hold them and what came before (append them first). Sequence b's tokens are rows query_starts[b] ..
     query_starts[b + 1] - 1 (int32 [batch + 1]), the last of them at position lengths[b] - 1. The rest as
-    paged_decode_attention; rows behind query_starts[-1] are left as they were (unset where `out` is made
+    paged_decode_attention; rows that belong to no sequence are left as they were (unset where `out` is made
     here)."""
-    cache, q_stride, out, out_stride, scale = _paged_attention_operands(q, k_cache, v_cache, page_table, lengths, scale, out)
-    tokens, q_heads, _ = q.shape
-    batch, columns = page_table.shape
-    _integers(query_starts, "query_starts", torch.int32, (batch + 1,), q.device)
-    _native.context(q.device).call(
-        "paged_prefill_attention", batch, tokens, q_heads, ct.byref(cache), page_table.data_ptr(), page_table.stride(0),
-        columns, lengths.data_ptr(), query_starts.data_ptr(), window, sinks, scale, q.data_ptr(), q_stride, out.data_ptr(),
-        out_stride)
-    return out
+    return _tensor_binding().paged_prefill_attention(q, k_cache, v_cache, page_table, lengths, query_starts, scale=scale,
+                                                     window=window, sinks=sinks, out=out)
 
 
 def decoder_layer_decode(hidden, residual, weights, k_cache, v_cache, positions, lengths, *,

@@ -79,4 +79,5 @@ Tensor linear_public(const Tensor &x, const Tensor &weight, const std::optional<
 void register_dense(pybind11::module_ &module);
 void register_fusion(pybind11::module_ &module);
 void register_quantized(pybind11::module_ &module);
+void register_paged(pybind11::module_ &module);
 } // namespace binding

@@ -27,7 +27,7 @@ namespace camblas_hip
 {
 namespace
 {
-constexpr int WAVES = 4, TILE = 32, HEADS = 16;
+constexpr int WAVES = 4, TILE = 32, HEADS = 16, JOIN_THREADS = 256, MOST_SHARES = 1024;
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct DecodeParams {
@@ -359,33 +359,71 @@ template <int DIM> __global__ __launch_bounds__(WAVES * 64, 2) void paged_decode
     }
 }
 
-// Joins the partials of one (heads, sequence) in the order of its positions; zeros where the sequence holds
-// nothing. One that a single workgroup held is written already.
-template <int DIM> __global__ __launch_bounds__(256) void paged_decode_join_kernel(DecodeParams p)
+// Joins the partials of one query head in the order of its positions; zeros where the sequence holds
+// nothing. A head that a single workgroup held is written already. All maxima are read at once, then DIM / 4
+// threads take a partial's row and the rows are dealt to the groups of threads: two trips to memory and an
+// ordered sum, whatever the number of partials (one thread per dim walking 64 of them took 140 us).
+template <int DIM> __global__ __launch_bounds__(JOIN_THREADS) void paged_decode_join_kernel(DecodeParams p)
 {
-    const int items = p.cache.kv_heads * p.head_tiles, sequence = blockIdx.y;
-    const Item item = item_of(p, sequence, blockIdx.x);
+    constexpr int ROW = DIM / 4, GROUPS = JOIN_THREADS / ROW, JOIN_WAVES = JOIN_THREADS / 64;
+    __shared__ float weight[MOST_SHARES], group_o[GROUPS][DIM], wave_top[JOIN_WAVES], wave_sums[JOIN_WAVES];
+    const int thread = threadIdx.x, lane = thread % 64, wave = thread / 64;
+    const int head = blockIdx.x, sequence = blockIdx.y, items = p.cache.kv_heads * p.head_tiles;
+    const int within = head % p.group, h = within % HEADS;
     int query;
     const bool empty = span_of(p, sequence, query).tiles == 0;
-    const int2 join = empty ? int2{0, 0} : p.joins[size_t(sequence) * items + blockIdx.x];
-    if (!empty && join.x == join.y)
+    unsigned short *out = p.out + int64_t(sequence) * p.out_stride + int64_t(head) * DIM;
+    if (empty) {
+        if (thread < DIM)
+            out[thread] = 0;
         return;
-    for (int index = threadIdx.x; index < item.heads * DIM; index += 256) {
-        const int h = index / DIM, d = index % DIM;
-        float best = -INFINITY, numerator = 0.f, denominator = 0.f;
-        if (!empty) {
-            for (int g = join.x; g <= join.y; ++g)
-                best = fmaxf(best, p.part_m[(2 * g + (g == join.x)) * HEADS + h]);
-            const float reference = best == -INFINITY ? 0.f : best;
-            for (int g = join.x; g <= join.y; ++g) {
-                const size_t row = size_t(2 * g + (g == join.x)) * HEADS + h;
-                const float factor = exp2f(p.part_m[row] - reference);
-                numerator = fmaf(factor, p.part_o[row * DIM + d], numerator);
-                denominator = fmaf(factor, p.part_l[row], denominator);
-            }
-        }
-        p.out[int64_t(sequence) * p.out_stride + int64_t(item.head0 + h) * DIM + d] =
-            float_to_bf16_bits(denominator == 0.f ? 0.f : numerator / denominator);
+    }
+    const int2 join = p.joins[size_t(sequence) * items + head / p.group * p.head_tiles + within / HEADS];
+    const int count = join.y - join.x + 1;
+    if (count == 1)
+        return;
+    const auto row_of = [&](int i) { return size_t(2 * (join.x + i) + (i == 0)) * HEADS + h; };
+    float top = -INFINITY;
+    for (int i = thread; i < count; i += JOIN_THREADS) {
+        const float m = p.part_m[row_of(i)];
+        weight[i] = m;
+        top = fmaxf(top, m);
+    }
+    top = wave_max(top);
+    if (lane == 0)
+        wave_top[wave] = top;
+    __syncthreads();
+    top = wave_top[0];
+#pragma unroll
+    for (int w = 1; w < JOIN_WAVES; ++w)
+        top = fmaxf(top, wave_top[w]);
+    const float reference = top == -INFINITY ? 0.f : top;
+    float sum = 0.f;
+    for (int i = thread; i < count; i += JOIN_THREADS) {
+        const float factor = __builtin_amdgcn_exp2f(weight[i] - reference);
+        weight[i] = factor;
+        sum = fmaf(factor, p.part_l[row_of(i)], sum);
+    }
+    sum = wave_sum(sum);
+    if (lane == 0)
+        wave_sums[wave] = sum;
+    __syncthreads();
+    const int group = thread / ROW, d = 4 * (thread % ROW);
+    f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int i = group; i < count; i += GROUPS)
+        o += weight[i] * *reinterpret_cast<const f32x4_t *>(p.part_o + row_of(i) * DIM + d);
+    *reinterpret_cast<f32x4_t *>(&group_o[group][d]) = o;
+    __syncthreads();
+    if (thread < DIM) {
+        float numerator = 0.f, denominator = 0.f;
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g)
+            numerator += group_o[g][thread];
+#pragma unroll
+        for (int w = 0; w < JOIN_WAVES; ++w)
+            denominator += wave_sums[w];
+        out[thread] = float_to_bf16_bits(denominator == 0.f ? 0.f : numerator / denominator);
     }
 }
 } // namespace
@@ -393,7 +431,7 @@ template <int DIM> __global__ __launch_bounds__(256) void paged_decode_join_kern
 // How a call is divided: workgroups that share all steps, or 0 for one workgroup per (heads, sequence).
 static int decode_shares(int64_t items, int64_t positions, int compute_units)
 {
-    const int64_t shares = 2 * int64_t(compute_units);
+    const int64_t shares = 2 * compute_units < MOST_SHARES ? 2 * compute_units : MOST_SHARES;
     if (positions <= 512 || items >= 4 * shares)
         return 0;
     return int(shares);
@@ -452,11 +490,11 @@ hipError_t launch_paged_decode(hipStream_t stream, int batch, int q_heads, int d
     hipError_t status = launch_status();
     if (status != hipSuccess)
         return status;
-    const dim3 grid(items, batch);
+    const dim3 grid(q_heads, batch);
     if (dim == 128)
-        paged_decode_join_kernel<128><<<grid, 256, 0, stream>>>(p);
+        paged_decode_join_kernel<128><<<grid, JOIN_THREADS, 0, stream>>>(p);
     else
-        paged_decode_join_kernel<64><<<grid, 256, 0, stream>>>(p);
+        paged_decode_join_kernel<64><<<grid, JOIN_THREADS, 0, stream>>>(p);
     return launch_status();
 }
 } // namespace camblas_hip

@@ -6,7 +6,7 @@
 // aten::mm.out and aten::addmm for the GPU dispatch key (ref: src/cuda/torch_backend.cuh:7-88).
 //
 // This unit holds the contexts, the tensor checks, the GEMM-shaped entry points and the module
-// definition; binding_dense.cpp, binding_fusion.cpp and binding_quantized.cpp hold the rest.
+// definition; binding_dense.cpp, binding_fusion.cpp, binding_quantized.cpp and binding_paged.cpp hold the rest.
 // PyTorch is used for device memory, the current stream and dispatch only; every product runs in
 // the library's own kernels. One library context exists per (thread, device, stream); a global
 // table lets `stats_all` and `close` reach the contexts of every thread.
@@ -533,6 +533,7 @@ PYBIND11_MODULE(_camblas_cuda_torch, module)
     register_dense(module);
     register_fusion(module);
     register_quantized(module);
+    register_paged(module);
     module.def("stats", &stats);
     module.def("stats_all", &stats_all);
     module.def("close", &close_all);

@@ -339,7 +339,7 @@ def test_empty_batches(device):
 
 
 def refused(call, *arguments, **options):
-    with pytest.raises((RuntimeError, ct.ArgumentError, TypeError)):
+    with pytest.raises((RuntimeError, ValueError, TypeError)):
         call(*arguments, **options)
 
 
@@ -404,7 +404,7 @@ def test_the_c_entry_refuses_a_small_or_missing_workspace(device):
     out = torch.zeros_like(q)
     held = torch.tensor(lengths, dtype=torch.int32, device=device)
     native = _native.context(device)
-    cache = _kernels._paged_cache(k, v, q)
+    cache = _native.PagedCache(k.data_ptr(), v.data_ptr(), *k.stride()[:3], *k.shape)
     columns = table.shape[1]
     size = _native.library().camblas_cuda_paged_decode_workspace_size(native.handle, 1, 4, ct.byref(cache), columns, 0, 0)
     assert size > 0
