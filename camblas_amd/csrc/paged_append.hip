@@ -69,7 +69,7 @@ __device__ __forceinline__ void unpack(const u32x4_t &packed, float (&x)[8])
 
 __device__ __forceinline__ u32x4_t pack(const float (&x)[8])
 {
-    return u32x4_t{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7])};
+    return u32x4_t{round_pair(x[0], x[1]), round_pair(x[2], x[3]), round_pair(x[4], x[5]), round_pair(x[6], x[7])};
 }
 
 template <int DIM> __global__ __launch_bounds__(APPEND_WAVES * 64) void qk_norm_rope_append_kernel(AppendParams p)

@@ -43,6 +43,14 @@ hipError_t launch_paged_prefill(hipStream_t stream, int batch, int tokens, int q
                                 const PageTable &table, const Visibility &see, const int32_t *starts, float scale,
                                 const void *q, int64_t q_stride, void *out, int64_t out_stride, int compute_units);
 
+// Two values to BF16 in one word, round to nearest even, NaN stays NaN: one instruction.
+__device__ __forceinline__ unsigned round_pair(float lo, float hi)
+{
+    typedef float pair_f32 __attribute__((ext_vector_type(2)));
+    typedef __bf16 pair_bf16 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(unsigned, __builtin_convertvector((pair_f32{lo, hi}), pair_bf16));
+}
+
 // The page of `position`, or -1 where the table or the cache has none.
 __device__ __forceinline__ int page_of(const PagedCache &cache, const int32_t *row, int columns, int position)
 {

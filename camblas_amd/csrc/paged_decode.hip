@@ -145,8 +145,8 @@ __device__ __forceinline__ void attend(const DecodeParams &p, Tile<DIM> &tile, c
             score[t][r] = __builtin_amdgcn_exp2f(score[t][r] - reference);
             run.total += score[t][r];
         }
-        weights[2 * t] = pack_bf16x2(score[t][0], score[t][1]);
-        weights[2 * t + 1] = pack_bf16x2(score[t][2], score[t][3]);
+        weights[2 * t] = round_pair(score[t][0], score[t][1]);
+        weights[2 * t + 1] = round_pair(score[t][2], score[t][3]);
     }
     const bf16x8_t p_frag = __builtin_bit_cast(bf16x8_t, weights);
 #pragma unroll

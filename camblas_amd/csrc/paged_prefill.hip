@@ -69,7 +69,7 @@ __device__ __forceinline__ int first_token(const PrefillParams &p, int sequence)
 }
 
 // COLS: 32-row column tiles per wavefront
-template <int DIM, int COLS> __global__ __launch_bounds__(WAVES * 64) void paged_prefill_kernel(PrefillParams p)
+template <int DIM, int COLS> __global__ __launch_bounds__(WAVES * 64, 2) void paged_prefill_kernel(PrefillParams p)
 {
     constexpr int ROWS = WAVES * COLS * 32, THREADS = WAVES * 64, CHUNKS = DIM / 8;
     constexpr int PIECES = TILE * CHUNKS / THREADS, PIECE_ROWS = THREADS / CHUNKS; // 16-byte chunks a thread moves
@@ -127,25 +127,30 @@ template <int DIM, int COLS> __global__ __launch_bounds__(WAVES * 64) void paged
     const int64_t head_at = int64_t(kv_head) * p.cache.head_stride;
     u32x4_t k_moving[PIECES], v_moving[PIECES];
     auto page_at = [&](int tile) {
+        // (-1 as well for a row that no query of the block sees)
         const int position = span.position(tile) + lane;
-        return position < span.end ? page_of(p.cache, pages, p.table.columns, position) : -1;
+        const bool wanted = position <= last_query &&
+                            (p.see.window <= 0 || position > first_query - p.see.window || position < p.see.sinks);
+        return wanted ? page_of(p.cache, pages, p.table.columns, position) : -1;
     };
     auto load = [&](int tile, int page) {
         const int base = span.position(tile);
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
             const int r = piece_row + i * PIECE_ROWS;
-            const int known = __shfl(page, r);
-            // (a row that holds nothing: zeros, which no weight turns into NaN)
-            k_moving[i] = v_moving[i] = u32x4_t{0, 0, 0, 0};
-            if (known >= 0) {
-                const int64_t at = row_offset(p.cache, known, base + r) + head_at + 8 * chunk;
-                k_moving[i] = *reinterpret_cast<const u32x4_t *>(p.cache.k + at);
-                v_moving[i] = *reinterpret_cast<const u32x4_t *>(p.cache.v + at);
-            }
+            const int known = __shfl(max(page, 0), r); // (a row that is not wanted: some row that exists)
+            const int64_t at = row_offset(p.cache, known, base + r) + head_at + 8 * chunk;
+            k_moving[i] = *reinterpret_cast<const u32x4_t *>(p.cache.k + at);
+            v_moving[i] = *reinterpret_cast<const u32x4_t *>(p.cache.v + at);
         }
     };
-    auto store = [&](int buffer) {
+    auto store = [&](int buffer, uint64_t wanted) {
+        if (wanted != ~uint64_t(0)) { // (uniform) zeros, which no weight turns into NaN
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i)
+                if (!((wanted >> (piece_row + i * PIECE_ROWS)) & 1))
+                    v_moving[i] = u32x4_t{0, 0, 0, 0};
+        }
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
             const int r = piece_row + i * PIECE_ROWS;
@@ -172,7 +177,7 @@ template <int DIM, int COLS> __global__ __launch_bounds__(WAVES * 64) void paged
         const int page = page_at(0);
         held = __ballot(page >= 0);
         load(0, page);
-        store(0);
+        store(0, held);
     }
     int next_page = span.tiles > 1 ? page_at(1) : -1;
     __syncthreads();
@@ -245,10 +250,10 @@ template <int DIM, int COLS> __global__ __launch_bounds__(WAVES * 64) void paged
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
                     weights[c][2 * t + u] = __builtin_bit_cast(
-                        bf16x8_t, u32x4_t{pack_bf16x2(score[c][t][8 * u], score[c][t][8 * u + 1]),
-                                          pack_bf16x2(score[c][t][8 * u + 2], score[c][t][8 * u + 3]),
-                                          pack_bf16x2(score[c][t][8 * u + 4], score[c][t][8 * u + 5]),
-                                          pack_bf16x2(score[c][t][8 * u + 6], score[c][t][8 * u + 7])});
+                        bf16x8_t, u32x4_t{round_pair(score[c][t][8 * u], score[c][t][8 * u + 1]),
+                                          round_pair(score[c][t][8 * u + 2], score[c][t][8 * u + 3]),
+                                          round_pair(score[c][t][8 * u + 4], score[c][t][8 * u + 5]),
+                                          round_pair(score[c][t][8 * u + 6], score[c][t][8 * u + 7])});
             }
         }
         // this lane points at position 16 u + 4 half + (lane % 16) / 4 (and eight further), dims of its sixteen
@@ -269,7 +274,7 @@ template <int DIM, int COLS> __global__ __launch_bounds__(WAVES * 64) void paged
                     acc[c][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, weights[c][u], acc[c][d], 0, 0, 0);
             }
         if (tile + 1 < span.tiles)
-            store(1 - buffer);
+            store(1 - buffer, next_held);
         held = next_held;
         __syncthreads();
     }
@@ -289,8 +294,8 @@ template <int DIM, int COLS> __global__ __launch_bounds__(WAVES * 64) void paged
 #pragma unroll
             for (int g = 0; g < 4; ++g)
                 *reinterpret_cast<u32x2_t *>(to + 32 * d + 8 * g) =
-                    u32x2_t{pack_bf16x2(acc[c][d][4 * g] * inverse, acc[c][d][4 * g + 1] * inverse),
-                            pack_bf16x2(acc[c][d][4 * g + 2] * inverse, acc[c][d][4 * g + 3] * inverse)};
+                    u32x2_t{round_pair(acc[c][d][4 * g] * inverse, acc[c][d][4 * g + 1] * inverse),
+                            round_pair(acc[c][d][4 * g + 2] * inverse, acc[c][d][4 * g + 3] * inverse)};
     }
 }
 } // namespace
