@@ -20,13 +20,14 @@
 // their sum is kept in FP32.
 #include "common.hpp"
 #include "device.hpp"
+#include "dma.hpp"
 #include "paged_cache.hpp"
 
 namespace camblas_hip
 {
 namespace
 {
-constexpr int WAVES = 4, TILE = 64;
+constexpr int WAVES = 4, THREADS = WAVES * 64, ROWS = WAVES * 32, TILE = 64;
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct PrefillParams {
@@ -43,39 +44,66 @@ struct PrefillParams {
 
 typedef short i16x4_t __attribute__((ext_vector_type(4)));
 typedef short i16x8_t __attribute__((ext_vector_type(8)));
-__device__ __forceinline__ i16x4_t gather_column(const unsigned short *address)
+__device__ __forceinline__ i16x4_t gather_column(const unsigned char *address)
 {
     return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4_t *)(address));
 }
 
-// Where 16-byte chunk `chunk` of tile row `row` lies, in elements. Keys: 16 (8 for 64 dims) consecutive rows
-// put a chunk on different banks. Values: pairs of chunks are moved, so that the four rows of a transposing
-// read lie on different banks.
-template <int DIM> __device__ __forceinline__ int key_slot(int row, int chunk)
+// Which 16-byte chunk of a tile's row lies at place `chunk`: the rows are turned so that reads meet no bank
+// twice. Keys are read as 16 rows of one chunk, values by transposing reads of 64 bytes of four rows.
+template <int DIM> __device__ __forceinline__ int turn_keys(int row)
 {
-    constexpr int CHUNKS = DIM / 8;
-    const int turned = CHUNKS == 16 ? row & 15 : ((row >> 1) & 7) ^ ((row & 1) << 2);
-    return (row * CHUNKS + (chunk ^ turned)) * 8;
+    return DIM == 128 ? row & 15 : ((row >> 1) & 7) ^ ((row & 1) << 2);
 }
-template <int DIM> __device__ __forceinline__ int value_slot(int row, int chunk)
+template <int DIM> __device__ __forceinline__ int turn_values(int row)
 {
-    constexpr int CHUNKS = DIM / 8;
-    return (row * CHUNKS + (chunk ^ (2 * (row & 3)))) * 8;
+    return DIM == 128 ? 4 * (row & 3) : 4 * ((row >> 1) & 1);
 }
+
+// 16 bytes per lane from base + offset (a lane's own, in bytes) or from a lane's own address to LDS at `to` +
+// 16 * lane, outside the compiler's bookkeeping: complete after a wait for vmcnt that the caller places. M0
+// is put back as it was, with the wait state that a load to LDS needs after a write of M0 on either side; a load
+// needs five after a vector instruction wrote the scalar registers of its address, which the compiler, not looking
+// into the text, does not see to.
+__device__ __forceinline__ void fetch_rows(const unsigned short *base, unsigned offset, const void *to)
+{
+    const uintptr_t address = reinterpret_cast<uintptr_t>(base);
+    const uint64_t uniform = (uint64_t(unsigned(__builtin_amdgcn_readfirstlane(unsigned(address >> 32)))) << 32) |
+                             unsigned(__builtin_amdgcn_readfirstlane(unsigned(address)));
+    const unsigned lds = __builtin_amdgcn_readfirstlane(static_cast<unsigned>(reinterpret_cast<uintptr_t>(to)));
+    unsigned saved;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 4\n\t"
+                 "global_load_lds_dwordx4 %2, %3\n\ts_mov_b32 m0, %0\n\ts_nop 0"
+                 : "=&s"(saved)
+                 : "s"(lds), "v"(offset), "s"(uniform)
+                 : "memory");
+}
+__device__ __forceinline__ void fetch_rows(const unsigned short *address, const void *to)
+{
+    const unsigned lds = __builtin_amdgcn_readfirstlane(static_cast<unsigned>(reinterpret_cast<uintptr_t>(to)));
+    unsigned saved;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\t"
+                 "global_load_lds_dwordx4 %2, off\n\ts_mov_b32 m0, %0\n\ts_nop 0"
+                 : "=&s"(saved)
+                 : "s"(lds), "v"(address)
+                 : "memory");
+}
+
+// a value that is the same in every lane, in a scalar register
+__device__ __forceinline__ int uniform(int value) { return __builtin_amdgcn_readfirstlane(value); }
 
 __device__ __forceinline__ int first_token(const PrefillParams &p, int sequence)
 {
     return min(max(p.starts[sequence], 0), p.tokens);
 }
 
-// COLS: 32-row column tiles per wavefront
-template <int DIM, int COLS> __global__ __launch_bounds__(WAVES * 64, 2) void paged_prefill_kernel(PrefillParams p)
+template <int DIM> __global__ __launch_bounds__(THREADS, 2) void paged_prefill_kernel(PrefillParams p)
 {
-    constexpr int ROWS = WAVES * COLS * 32, THREADS = WAVES * 64, CHUNKS = DIM / 8;
-    constexpr int PIECES = TILE * CHUNKS / THREADS, PIECE_ROWS = THREADS / CHUNKS; // 16-byte chunks a thread moves
-    __shared__ __attribute__((aligned(16))) unsigned short key_tile[2][TILE * DIM], value_tile[2][TILE * DIM];
+    constexpr int CHUNKS = DIM / 8, FETCH = 64 / CHUNKS, FETCHES = TILE / FETCH / WAVES; // rows of a load, a wavefront's loads
+    __shared__ __attribute__((aligned(16))) unsigned char keys0[TILE * DIM * 2], keys1[TILE * DIM * 2];
+    __shared__ __attribute__((aligned(16))) unsigned char values0[TILE * DIM * 2], values1[TILE * DIM * 2];
     __shared__ int found;
-    const int thread = threadIdx.x, lane = thread % 64, wave = thread / 64;
+    const int thread = threadIdx.x, lane = thread % 64, wave = uniform(thread / 64);
     const int column = lane % 32, half = lane / 32;
     // the last blocks of a causal sequence see most: they start first
     const int kv_head = int(blockIdx.x) % p.cache.kv_heads;
@@ -95,208 +123,225 @@ template <int DIM, int COLS> __global__ __launch_bounds__(WAVES * 64, 2) void pa
     }
     __syncthreads();
     const int sequence = __builtin_amdgcn_readfirstlane(found);
-    const int token0 = first_token(p, sequence), tokens = first_token(p, sequence + 1) - token0;
+    const int token0 = uniform(first_token(p, sequence)), tokens = uniform(first_token(p, sequence + 1)) - token0;
     const int64_t row0 = (block - (int64_t(token0) * p.group / ROWS + sequence)) * ROWS;
     const int64_t rows = int64_t(tokens) * p.group - row0;
     if (row0 < 0 || rows <= 0)
         return;
 
-    // ---- this lane's rows: token and query head, position
-    const int length = live_positions(p.table, p.cache, sequence);
-    const int past = length - tokens;
-    int query[COLS];
-    bf16x8_t q[COLS][DIM / 16];
-#pragma unroll
-    for (int c = 0; c < COLS; ++c) {
-        const int64_t row = row0 + (wave * COLS + c) * 32 + column;
+    // ---- this lane's row: token and query head, position
+    const int past = uniform(live_positions(p.table, p.cache, sequence)) - tokens;
+    int query;
+    bf16x8_t q[DIM / 16];
+    {
+        const int64_t row = row0 + wave * 32 + column;
         const int64_t kept = row < rows + row0 ? row : rows + row0 - 1;
         const int token = int(kept / p.group), head = kv_head * p.group + int(kept % p.group);
-        query[c] = past + token;
+        query = past + token;
         const unsigned short *from = p.q + int64_t(token0 + token) * p.q_stride + int64_t(head) * DIM + 8 * half;
 #pragma unroll
         for (int s = 0; s < DIM / 16; ++s)
-            q[c][s] = *reinterpret_cast<const bf16x8_t *>(from + 16 * s);
+            q[s] = *reinterpret_cast<const bf16x8_t *>(from + 16 * s);
     }
-    const int first_query = past + int(row0 / p.group);
-    const int last_query = past + int((row0 + min(rows, int64_t(ROWS)) - 1) / p.group);
+    const int first_query = uniform(past + int(row0 / p.group));
+    const int last_query = uniform(past + int((row0 + min(rows, int64_t(ROWS)) - 1) / p.group));
     const TileSpan<TILE> span(p.see, first_query, last_query);
 
-    // ---- moving tiles: lane r of every wavefront knows the page of tile row r
+    // ---- fetching tiles: lane r of every wavefront knows the page of tile row r
     const int32_t *pages = p.table.pages + int64_t(sequence) * p.table.stride;
-    const int chunk = thread % CHUNKS, piece_row = thread / CHUNKS;
-    const int64_t head_at = int64_t(kv_head) * p.cache.head_stride;
-    u32x4_t k_moving[PIECES], v_moving[PIECES];
-    auto page_at = [&](int tile) {
-        // (-1 as well for a row that no query of the block sees)
+    const auto page_at = [&](int tile) {
+        return tile < span.tiles ? page_of(p.cache, pages, p.table.columns, span.position(tile) + lane) : -1;
+    };
+    // which rows of a tile exist and are seen by some query of the block
+    const auto wanted_rows = [&](int tile, int page) {
         const int position = span.position(tile) + lane;
-        const bool wanted = position <= last_query &&
-                            (p.see.window <= 0 || position > first_query - p.see.window || position < p.see.sinks);
-        return wanted ? page_of(p.cache, pages, p.table.columns, position) : -1;
+        return __ballot(page >= 0 && position <= last_query &&
+                        (p.see.window <= 0 || position > first_query - p.see.window || position < p.see.sinks));
     };
-    auto load = [&](int tile, int page) {
+    // Load i of a wavefront brings rows FETCH * wave + FETCH * WAVES * i and the FETCH - 1 after it, in the order
+    // of their turned chunks; which chunk a lane brings is the same for every load.
+    const int fetch_row = FETCH * wave + lane / CHUNKS;
+    const unsigned key_chunk = unsigned((lane % CHUNKS) ^ turn_keys<DIM>(fetch_row)) * 8;
+    const unsigned value_chunk = unsigned((lane % CHUNKS) ^ turn_values<DIM>(fetch_row)) * 8;
+    const int64_t head_at = int64_t(kv_head) * p.cache.head_stride;
+    const bool pages_hold_loads = (1 << p.cache.page_shift) >= FETCH;
+    const unsigned row_bytes = unsigned(lane / CHUNKS) * unsigned(pages_hold_loads ? p.cache.slot_stride : 0) * 2;
+    const auto fetch = [&](const unsigned short *array, unsigned chunk, int tile, int page, unsigned char *to) {
         const int base = span.position(tile);
+        const int known = max(page, 0); // (a row that does not exist: some row that does, and is not used)
 #pragma unroll
-        for (int i = 0; i < PIECES; ++i) {
-            const int r = piece_row + i * PIECE_ROWS;
-            const int known = __shfl(max(page, 0), r); // (a row that is not wanted: some row that exists)
-            const int64_t at = row_offset(p.cache, known, base + r) + head_at + 8 * chunk;
-            k_moving[i] = *reinterpret_cast<const u32x4_t *>(p.cache.k + at);
-            v_moving[i] = *reinterpret_cast<const u32x4_t *>(p.cache.v + at);
-        }
-    };
-    auto store = [&](int buffer, uint64_t wanted) {
-        if (wanted != ~uint64_t(0)) { // (uniform) zeros, which no weight turns into NaN
-#pragma unroll
-            for (int i = 0; i < PIECES; ++i)
-                if (!((wanted >> (piece_row + i * PIECE_ROWS)) & 1))
-                    v_moving[i] = u32x4_t{0, 0, 0, 0};
-        }
-#pragma unroll
-        for (int i = 0; i < PIECES; ++i) {
-            const int r = piece_row + i * PIECE_ROWS;
-            *reinterpret_cast<u32x4_t *>(&key_tile[buffer][key_slot<DIM>(r, chunk)]) = k_moving[i];
-            *reinterpret_cast<u32x4_t *>(&value_tile[buffer][value_slot<DIM>(r, chunk)]) = v_moving[i];
+        for (int i = 0; i < FETCHES; ++i) {
+            const int first = FETCH * wave + FETCH * WAVES * i;
+            if (pages_hold_loads) { // (uniform)
+                const int64_t at = row_offset(p.cache, __builtin_amdgcn_readlane(known, first), base + first) + head_at;
+                fetch_rows(array + at, row_bytes + 2 * chunk, to + first * DIM * 2);
+            } else {
+                const int r = first + lane / CHUNKS;
+                const int64_t at = row_offset(p.cache, __shfl(known, r), base + r) + head_at + chunk;
+                fetch_rows(array + at, to + first * DIM * 2);
+            }
         }
     };
 
-    f32x16_t acc[COLS][DIM / 32];
-    float top[COLS], total[COLS];
+    // ---- reading tiles
+    int key_at[DIM / 16], value_at[DIM / 32]; // byte offsets of this lane's operands
 #pragma unroll
-    for (int c = 0; c < COLS; ++c) {
-        top[c] = -INFINITY;
-        total[c] = 0.f;
+    for (int s = 0; s < DIM / 16; ++s)
+        key_at[s] = column * DIM * 2 + ((2 * s + half) ^ turn_keys<DIM>(column)) * 16;
+    {
+        const int spot = 4 * half + lane % 16 / 4; // (position 16 u + spot, and eight further)
 #pragma unroll
-        for (int d = 0; d < DIM / 32; ++d)
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-                acc[c][d][r] = 0.f;
-    }
-
-    uint64_t held = 0, next_held = 0; // which rows of a tile exist
-    if (span.tiles > 0) {
-        const int page = page_at(0);
-        held = __ballot(page >= 0);
-        load(0, page);
-        store(0, held);
-    }
-    int next_page = span.tiles > 1 ? page_at(1) : -1;
-    __syncthreads();
-    for (int tile = 0; tile < span.tiles; ++tile) {
-        const int buffer = tile & 1, base = span.position(tile);
-        if (tile + 1 < span.tiles) {
-            next_held = __ballot(next_page >= 0);
-            load(tile + 1, next_page);
-            if (tile + 2 < span.tiles)
-                next_page = page_at(tile + 2);
+        for (int d = 0; d < DIM / 32; ++d) {
+            const int dim = 32 * d + 16 * (lane / 16 % 2) + 4 * (lane % 4);
+            value_at[d] = spot * DIM * 2 + ((dim / 8) ^ turn_values<DIM>(spot)) * 16 + dim % 8 * 2;
         }
-        const bool whole = held == ~uint64_t(0) && base + TILE - 1 <= first_query &&
-                           (p.see.window <= 0 || base > last_query - p.see.window || base + TILE <= p.see.sinks);
-
-        f32x16_t score[COLS][2];
+    }
+    const auto multiply_keys = [&](const unsigned char *tile, f32x16_t (&score)[2]) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
 #pragma unroll
-            for (int c = 0; c < COLS; ++c)
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    score[c][t][r] = 0.f;
+            for (int r = 0; r < 16; ++r)
+                score[t][r] = 0.f;
 #pragma unroll
             for (int s = 0; s < DIM / 16; ++s) {
-                const bf16x8_t k =
-                    *reinterpret_cast<const bf16x8_t *>(&key_tile[buffer][key_slot<DIM>(32 * t + column, 2 * s + half)]);
-#pragma unroll
-                for (int c = 0; c < COLS; ++c)
-                    score[c][t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, q[c][s], score[c][t], 0, 0, 0);
+                const bf16x8_t k = *reinterpret_cast<const bf16x8_t *>(tile + key_at[s] + 32 * t * DIM * 2);
+                score[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, q[s], score[t], 0, 0, 0);
             }
         }
-        bf16x8_t weights[COLS][4];
+    };
+
+    f32x16_t acc[DIM / 32];
+    float top = -INFINITY, total = 0.f;
 #pragma unroll
-        for (int c = 0; c < COLS; ++c) {
-            if (!whole) {
+    for (int d = 0; d < DIM / 32; ++d)
 #pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int at = 32 * t + 8 * (r / 4) + 4 * half + r % 4;
-                        if (!((held >> at) & 1) || !sees(p.see, query[c], base + at))
-                            score[c][t][r] = -INFINITY;
-                    }
-            }
-            float highest = -INFINITY;
+        for (int r = 0; r < 16; ++r)
+            acc[d][r] = 0.f;
+
+    // Turn `tile`: its scores are in `score`, its values in `values`, the keys of the next tile in `next_keys`.
+    // Fetched meanwhile: the next tile's values, the keys of the one after. The next tile's scores are multiplied
+    // while this one's weights are worked out.
+    uint64_t wanted;
+    int page;
+    const auto turn = [&](int tile, f32x16_t (&score)[2], f32x16_t (&next_score)[2], unsigned char *keys,
+                          const unsigned char *next_keys, unsigned char *values, unsigned char *next_values) {
+        const int base = span.position(tile);
+        const uint64_t next_wanted = wanted_rows(tile + 1, page);
+        if (tile + 1 < span.tiles)
+            fetch(p.cache.v, value_chunk, tile + 1, page, next_values);
+        page = page_at(tile + 2);
+        if (tile + 2 < span.tiles)
+            fetch(p.cache.k, key_chunk, tile + 2, page, keys);
+        const bool whole = wanted == ~uint64_t(0) && base + TILE - 1 <= first_query &&
+                           (p.see.window <= 0 || base > last_query - p.see.window || base + TILE <= p.see.sinks);
+        if (!whole) { // (the same in every wavefront)
+            // position base + 4 half + at, against what the lane's query sees, as comparisons with constants
+            const uint64_t here = wanted >> (4 * half);
+            const int last = query - base - 4 * half, first = p.see.window > 0 ? last - p.see.window : -TILE;
+            const int sinks = p.see.window > 0 ? p.see.sinks - base - 4 * half : 0;
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    highest = fmaxf(highest, score[c][t][r]);
-            highest *= p.scale;
-            if (__any(highest > top[c] + 8.f)) {
-                highest = fmaxf(highest, __shfl_xor(highest, 32));
-                highest = fmaxf(highest, top[c]);
-                const float factor = top[c] == highest ? 1.f : __builtin_amdgcn_exp2f(top[c] - highest);
-                top[c] = highest;
-                total[c] *= factor;
-#pragma unroll
-                for (int d = 0; d < DIM / 32; ++d)
-                    acc[c][d] *= factor;
-            }
-            const float reference = top[c] == -INFINITY ? 0.f : top[c];
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-#pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    score[c][t][r] = __builtin_amdgcn_exp2f(fmaf(score[c][t][r], p.scale, -reference));
-                    total[c] += score[c][t][r];
+                    const int at = 32 * t + 8 * (r / 4) + r % 4;
+                    const bool seen = ((here >> at) & 1) && at <= last && (at > first || at < sinks);
+                    score[t][r] = seen ? score[t][r] : -INFINITY;
                 }
-#pragma unroll
-                for (int u = 0; u < 2; ++u)
-                    weights[c][2 * t + u] = __builtin_bit_cast(
-                        bf16x8_t, u32x4_t{round_pair(score[c][t][8 * u], score[c][t][8 * u + 1]),
-                                          round_pair(score[c][t][8 * u + 2], score[c][t][8 * u + 3]),
-                                          round_pair(score[c][t][8 * u + 4], score[c][t][8 * u + 5]),
-                                          round_pair(score[c][t][8 * u + 6], score[c][t][8 * u + 7])});
-            }
+            // rows that nobody sees: zeros, which no weight turns into NaN
+            for (int piece = thread; piece < TILE * CHUNKS; piece += THREADS)
+                if (!((wanted >> (piece / CHUNKS)) & 1))
+                    *reinterpret_cast<u32x4_t *>(values + piece * 16) = u32x4_t{0, 0, 0, 0};
+            __syncthreads();
         }
-        // this lane points at position 16 u + 4 half + (lane % 16) / 4 (and eight further), dims of its sixteen
-        const int spot = 4 * half + (lane % 16) / 4;
+        float highest = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                highest = fmaxf(highest, score[t][r]);
+        highest *= p.scale;
+        if (__any(highest > top + 8.f)) {
+            highest = fmaxf(highest, __shfl_xor(highest, 32));
+            highest = fmaxf(highest, top);
+            const float factor = top == highest ? 1.f : __builtin_amdgcn_exp2f(top - highest);
+            top = highest;
+            total *= factor;
+#pragma unroll
+            for (int d = 0; d < DIM / 32; ++d)
+                acc[d] *= factor;
+        }
+        const float reference = top == -INFINITY ? 0.f : top;
+        multiply_keys(next_keys, next_score);
+        bf16x8_t weights[4];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                score[t][r] = __builtin_amdgcn_exp2f(fmaf(score[t][r], p.scale, -reference));
+                total += score[t][r];
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+                weights[2 * t + u] = __builtin_bit_cast(
+                    bf16x8_t, u32x4_t{round_pair(score[t][8 * u], score[t][8 * u + 1]),
+                                      round_pair(score[t][8 * u + 2], score[t][8 * u + 3]),
+                                      round_pair(score[t][8 * u + 4], score[t][8 * u + 5]),
+                                      round_pair(score[t][8 * u + 6], score[t][8 * u + 7])});
+        }
 #pragma unroll
         for (int u = 0; u < TILE / 16; ++u)
 #pragma unroll
             for (int d = 0; d < DIM / 32; ++d) {
-                const int dims = 32 * d + 16 * (lane / 16 % 2) + 4 * (lane % 4);
-                const i16x4_t lower =
-                    gather_column(&value_tile[buffer][value_slot<DIM>(16 * u + spot, dims / 8) + dims % 8]);
-                const i16x4_t upper =
-                    gather_column(&value_tile[buffer][value_slot<DIM>(16 * u + 8 + spot, dims / 8) + dims % 8]);
+                const i16x4_t lower = gather_column(values + value_at[d] + 16 * u * DIM * 2);
+                const i16x4_t upper = gather_column(values + value_at[d] + (16 * u + 8) * DIM * 2);
                 const bf16x8_t v = __builtin_bit_cast(
                     bf16x8_t, i16x8_t{lower[0], lower[1], lower[2], lower[3], upper[0], upper[1], upper[2], upper[3]});
-#pragma unroll
-                for (int c = 0; c < COLS; ++c)
-                    acc[c][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, weights[c][u], acc[c][d], 0, 0, 0);
+                acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, weights[u], acc[d], 0, 0, 0);
             }
-        if (tile + 1 < span.tiles)
-            store(1 - buffer, next_held);
-        held = next_held;
-        __syncthreads();
+        wanted = next_wanted;
+        asm volatile("" ::: "memory");
+        pipeline_barrier<0>();
+        asm volatile("" ::: "memory");
+    };
+
+    if (span.tiles > 0) {
+        page = page_at(0);
+        wanted = wanted_rows(0, page);
+        fetch(p.cache.k, key_chunk, 0, page, keys0);
+        fetch(p.cache.v, value_chunk, 0, page, values0);
+        page = page_at(1);
+        if (span.tiles > 1)
+            fetch(p.cache.k, key_chunk, 1, page, keys1);
+        pipeline_barrier<0>();
+        asm volatile("" ::: "memory");
+        f32x16_t even[2], odd[2];
+        multiply_keys(keys0, even);
+        asm volatile("" ::: "memory");
+        pipeline_barrier<0>();
+        asm volatile("" ::: "memory");
+        for (int tile = 0; tile < span.tiles; tile += 2) {
+            turn(tile, even, odd, keys0, keys1, values0, values1);
+            if (tile + 1 >= span.tiles)
+                break;
+            turn(tile + 1, odd, even, keys1, keys0, values1, values0);
+        }
     }
 
+    const int64_t row = row0 + wave * 32 + column;
+    const float sum = total + __shfl_xor(total, 32);
+    if (row >= row0 + rows)
+        return;
+    // (no position seen: zero; a sum that is NaN stays NaN)
+    const float inverse = sum == 0.f ? 0.f : 1.f / sum;
+    const int token = token0 + int(row / p.group), head = kv_head * p.group + int(row % p.group);
+    unsigned short *to = p.out + int64_t(token) * p.out_stride + int64_t(head) * DIM + 4 * half;
 #pragma unroll
-    for (int c = 0; c < COLS; ++c) {
-        const int64_t row = row0 + (wave * COLS + c) * 32 + column;
-        const float sum = total[c] + __shfl_xor(total[c], 32);
-        if (row >= row0 + rows)
-            continue;
-        // (no position seen: zero; a sum that is NaN stays NaN)
-        const float inverse = sum == 0.f ? 0.f : 1.f / sum;
-        const int token = token0 + int(row / p.group), head = kv_head * p.group + int(row % p.group);
-        unsigned short *to = p.out + int64_t(token) * p.out_stride + int64_t(head) * DIM + 4 * half;
+    for (int d = 0; d < DIM / 32; ++d)
 #pragma unroll
-        for (int d = 0; d < DIM / 32; ++d)
-#pragma unroll
-            for (int g = 0; g < 4; ++g)
-                *reinterpret_cast<u32x2_t *>(to + 32 * d + 8 * g) =
-                    u32x2_t{round_pair(acc[c][d][4 * g] * inverse, acc[c][d][4 * g + 1] * inverse),
-                            round_pair(acc[c][d][4 * g + 2] * inverse, acc[c][d][4 * g + 3] * inverse)};
-    }
+        for (int g = 0; g < 4; ++g)
+            *reinterpret_cast<u32x2_t *>(to + 32 * d + 8 * g) =
+                u32x2_t{round_pair(acc[d][4 * g] * inverse, acc[d][4 * g + 1] * inverse),
+                        round_pair(acc[d][4 * g + 2] * inverse, acc[d][4 * g + 3] * inverse)};
 }
 } // namespace
 
@@ -304,7 +349,6 @@ hipError_t launch_paged_prefill(hipStream_t stream, int batch, int tokens, int q
                                 const PageTable &table, const Visibility &see, const int32_t *starts, float scale,
                                 const void *q, int64_t q_stride, void *out, int64_t out_stride, int compute_units)
 {
-    constexpr int COLS = 1, ROWS = WAVES * COLS * 32;
     PrefillParams p = {};
     p.batch = batch;
     p.tokens = tokens;
@@ -324,9 +368,9 @@ hipError_t launch_paged_prefill(hipStream_t stream, int batch, int tokens, int q
     p.out_stride = out_stride;
     const unsigned grid = unsigned(blocks * cache.kv_heads);
     if (dim == 128)
-        paged_prefill_kernel<128, COLS><<<grid, WAVES * 64, 0, stream>>>(p);
+        paged_prefill_kernel<128><<<grid, WAVES * 64, 0, stream>>>(p);
     else
-        paged_prefill_kernel<64, COLS><<<grid, WAVES * 64, 0, stream>>>(p);
+        paged_prefill_kernel<64><<<grid, WAVES * 64, 0, stream>>>(p);
     return launch_status();
 }
 } // namespace camblas_hip
