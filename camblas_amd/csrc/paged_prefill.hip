@@ -61,25 +61,38 @@ template <int DIM> __device__ __forceinline__ int turn_values(int row)
     return DIM == 128 ? 4 * (row & 3) : 4 * ((row >> 1) & 1);
 }
 
-// 16 bytes per lane from base + offset (a lane's own, in bytes) or from a lane's own address to LDS at `to` +
-// 16 * lane, outside the compiler's bookkeeping: complete after a wait for vmcnt that the caller places. M0
-// is put back as it was, with the wait state that a load to LDS needs after a write of M0 on either side; a load
-// needs five after a vector instruction wrote the scalar registers of its address, which the compiler, not looking
-// into the text, does not see to.
-__device__ __forceinline__ void fetch_rows(const unsigned short *base, unsigned offset, const void *to)
+// Loads to LDS outside the compiler's bookkeeping, complete after a wait for vmcnt that the caller places:
+// 16 bytes per lane and load, load i to `to` + 1024 i + 16 * lane. M0 is put back as it was; a load to LDS
+// needs a wait state after a write of M0, and five after a vector instruction wrote the scalar registers of
+// its address, which the compiler, not looking into the text, does not see to.
+// The first form reads from base (the same in every lane) + a lane's own offsets in bytes.
+template <int LOADS> __device__ __forceinline__ void fetch_rows(const unsigned short *base, const unsigned (&offset)[LOADS], const void *to)
 {
+    static_assert(LOADS == 2 || LOADS == 4, "a wavefront's share of a tile");
     const uintptr_t address = reinterpret_cast<uintptr_t>(base);
     const uint64_t uniform = (uint64_t(unsigned(__builtin_amdgcn_readfirstlane(unsigned(address >> 32)))) << 32) |
                              unsigned(__builtin_amdgcn_readfirstlane(unsigned(address)));
     const unsigned lds = __builtin_amdgcn_readfirstlane(static_cast<unsigned>(reinterpret_cast<uintptr_t>(to)));
     unsigned saved;
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 4\n\t"
-                 "global_load_lds_dwordx4 %2, %3\n\ts_mov_b32 m0, %0\n\ts_nop 0"
-                 : "=&s"(saved)
-                 : "s"(lds), "v"(offset), "s"(uniform)
-                 : "memory");
+    if constexpr (LOADS == 4)
+        asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 4\n\t"
+                     "global_load_lds_dwordx4 %2, %6\n\ts_add_u32 m0, m0, 0x400\n\ts_nop 0\n\t"
+                     "global_load_lds_dwordx4 %3, %6\n\ts_add_u32 m0, m0, 0x400\n\ts_nop 0\n\t"
+                     "global_load_lds_dwordx4 %4, %6\n\ts_add_u32 m0, m0, 0x400\n\ts_nop 0\n\t"
+                     "global_load_lds_dwordx4 %5, %6\n\ts_mov_b32 m0, %0\n\ts_nop 0"
+                     : "=&s"(saved)
+                     : "s"(lds), "v"(offset[0]), "v"(offset[1]), "v"(offset[LOADS - 2]), "v"(offset[LOADS - 1]), "s"(uniform)
+                     : "memory", "scc");
+    else
+        asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 4\n\t"
+                     "global_load_lds_dwordx4 %2, %4\n\ts_add_u32 m0, m0, 0x400\n\ts_nop 0\n\t"
+                     "global_load_lds_dwordx4 %3, %4\n\ts_mov_b32 m0, %0\n\ts_nop 0"
+                     : "=&s"(saved)
+                     : "s"(lds), "v"(offset[0]), "v"(offset[1]), "s"(uniform)
+                     : "memory", "scc");
 }
-__device__ __forceinline__ void fetch_rows(const unsigned short *address, const void *to)
+// One load from a lane's own address.
+__device__ __forceinline__ void fetch_row(const unsigned short *address, const void *to)
 {
     const unsigned lds = __builtin_amdgcn_readfirstlane(static_cast<unsigned>(reinterpret_cast<uintptr_t>(to)));
     unsigned saved;
@@ -165,27 +178,33 @@ template <int DIM> __global__ __launch_bounds__(THREADS, DIM == 64 ? 3 : 2) void
         return __ballot(page >= 0 && position <= last_query &&
                         (p.see.window <= 0 || position > first_query - p.see.window || position < p.see.sinks));
     };
-    // Load i of a wavefront brings rows FETCH * wave + FETCH * WAVES * i and the FETCH - 1 after it, in the order
-    // of their turned chunks; which chunk a lane brings is the same for every load.
-    const int fetch_row = FETCH * wave + lane / CHUNKS;
-    const unsigned key_chunk = unsigned((lane % CHUNKS) ^ turn_keys<DIM>(fetch_row)) * 8;
-    const unsigned value_chunk = unsigned((lane % CHUNKS) ^ turn_values<DIM>(fetch_row)) * 8;
+    // A wavefront brings rows 16 * wave .. + 15, FETCH of them with a load, in the order of their turned chunks. Where
+    // pages hold at least 16 rows those lie in one page, at offsets that are the same for every tile.
+    const int own_row = 16 * wave;
+    const bool one_page = (16 >> p.cache.page_shift) <= 1 && p.cache.slot_stride < (int64_t(1) << 26);
     const int64_t head_at = int64_t(kv_head) * p.cache.head_stride;
-    const bool pages_hold_loads = (1 << p.cache.page_shift) >= FETCH;
-    const unsigned row_bytes = unsigned(lane / CHUNKS) * unsigned(pages_hold_loads ? p.cache.slot_stride : 0) * 2;
-    const auto fetch = [&](const unsigned short *array, unsigned chunk, int tile, int page, unsigned char *to) {
-        const int base = span.position(tile);
-        const int known = max(page, 0); // (a row that does not exist: some row that does, and is not used)
+    unsigned key_from[FETCHES], value_from[FETCHES]; // bytes
 #pragma unroll
-        for (int i = 0; i < FETCHES; ++i) {
-            const int first = FETCH * wave + FETCH * WAVES * i;
-            if (pages_hold_loads) { // (uniform)
-                const int64_t at = row_offset(p.cache, __builtin_amdgcn_readlane(known, first), base + first) + head_at;
-                fetch_rows(array + at, row_bytes + 2 * chunk, to + first * DIM * 2);
-            } else {
-                const int r = first + lane / CHUNKS;
-                const int64_t at = row_offset(p.cache, __shfl(known, r), base + r) + head_at + chunk;
-                fetch_rows(array + at, to + first * DIM * 2);
+    for (int i = 0; i < FETCHES; ++i) {
+        const int r = FETCH * i + lane / CHUNKS;
+        const unsigned along = one_page ? unsigned(r) * unsigned(p.cache.slot_stride) * 2 : 0;
+        key_from[i] = along + unsigned((lane % CHUNKS) ^ turn_keys<DIM>(r)) * 16;
+        value_from[i] = along + unsigned((lane % CHUNKS) ^ turn_values<DIM>(r)) * 16;
+    }
+    // where the wavefront's first row of a tile lies (a row that does not exist: some row that does, and is not used)
+    const auto place = [&](int tile, int page) {
+        return row_offset(p.cache, max(__builtin_amdgcn_readlane(page, own_row), 0), span.position(tile) + own_row) + head_at;
+    };
+    const auto fetch = [&](const unsigned short *array, const unsigned (&from)[FETCHES], int64_t at, int tile, int page,
+                           unsigned char *to) {
+        if (one_page) { // (uniform)
+            fetch_rows(array + at, from, to + own_row * DIM * 2);
+        } else {
+#pragma unroll
+            for (int i = 0; i < FETCHES; ++i) {
+                const int r = own_row + FETCH * i + lane / CHUNKS;
+                const int64_t own = row_offset(p.cache, max(__shfl(page, r), 0), span.position(tile) + r) + head_at;
+                fetch_row(array + own + from[i] / 2, to + (own_row + FETCH * i) * DIM * 2);
             }
         }
     };
@@ -229,16 +248,20 @@ template <int DIM> __global__ __launch_bounds__(THREADS, DIM == 64 ? 3 : 2) void
     // Fetched meanwhile: the next tile's values, the keys of the one after. The next tile's scores are multiplied
     // while this one's weights are worked out.
     uint64_t wanted;
-    int page;
+    int page, next_page; // of the rows of the next tile and of the one after
+    int64_t at = 0;      // place() of the next tile
     const auto turn = [&](int tile, f32x16_t (&score)[2], f32x16_t (&next_score)[2], unsigned char *keys,
                           const unsigned char *next_keys, unsigned char *values, unsigned char *next_values) {
         const int base = span.position(tile);
         const uint64_t next_wanted = wanted_rows(tile + 1, page);
         if (tile + 1 < span.tiles)
-            fetch(p.cache.v, value_chunk, tile + 1, page, next_values);
-        page = page_at(tile + 2);
-        if (tile + 2 < span.tiles)
-            fetch(p.cache.k, key_chunk, tile + 2, page, keys);
+            fetch(p.cache.v, value_from, at, tile + 1, page, next_values);
+        page = next_page;
+        if (tile + 2 < span.tiles) {
+            at = place(tile + 2, page);
+            fetch(p.cache.k, key_from, at, tile + 2, page, keys);
+        }
+        next_page = page_at(tile + 3);
         const bool whole = wanted == ~uint64_t(0) && base + TILE - 1 <= first_query &&
                            (p.see.window <= 0 || base > last_query - p.see.window || base + TILE <= p.see.sinks);
         if (!whole) { // (the same in every wavefront)
@@ -331,11 +354,15 @@ template <int DIM> __global__ __launch_bounds__(THREADS, DIM == 64 ? 3 : 2) void
     if (span.tiles > 0) {
         page = page_at(0);
         wanted = wanted_rows(0, page);
-        fetch(p.cache.k, key_chunk, 0, page, keys0);
-        fetch(p.cache.v, value_chunk, 0, page, values0);
+        at = place(0, page);
+        fetch(p.cache.k, key_from, at, 0, page, keys0);
+        fetch(p.cache.v, value_from, at, 0, page, values0);
         page = page_at(1);
-        if (span.tiles > 1)
-            fetch(p.cache.k, key_chunk, 1, page, keys1);
+        next_page = page_at(2);
+        if (span.tiles > 1) {
+            at = place(1, page);
+            fetch(p.cache.k, key_from, at, 1, page, keys1);
+        }
         pipeline_barrier<0>();
         asm volatile("" ::: "memory");
         f32x16_t even[2], odd[2];
