@@ -55,73 +55,96 @@ template <int DIM> struct Running {
     float top, total;
 };
 
-template <int DIM> struct Tile {
-    bf16x8_t k[2][DIM / 32];
-    unsigned v[8][DIM / 32]; // DIM / 16 values of each of eight positions
-    unsigned mask;           // which of the 32 positions the token sees
-};
-
-template <int DIM>
 __device__ __forceinline__ int fetch_page(const DecodeParams &p, const int32_t *row, int base, int lane)
 {
     return page_of(p.cache, row, p.table.columns, base + lane % TILE);
 }
 
+// Eight rows of a tile for every lane, 16 lanes to a row: rows 16 (e / 4) + 4 j + e % 4, DIM / 16 values from
+// (DIM / 16) m on. Every row is read once and by one load: it takes no place in the caches.
+// LARGE: pages of 16 positions and more, so that each half of a tile lies in one page: its place is then the
+// same in every lane, and a lane's own offsets (`along`, in bytes, for the rows 4 j + 0 .. 3) the same in
+// every tile. page: lane r holds that of row r % 32; a row without one is read from some page that exists, and not used.
+template <int DIM, bool LARGE>
+__device__ __forceinline__ void load_rows(const DecodeParams &p, const unsigned short *array, int base, int page, int64_t head,
+                                          int lane, u32x4_t along, unsigned (&rows)[8][DIM / 32])
+{
+    typedef unsigned row_t __attribute__((ext_vector_type(DIM / 32)));
+    const int known = page < 0 ? 0 : page;
+    row_t got[8];
+    if constexpr (LARGE) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int64_t at = row_offset(p.cache, __builtin_amdgcn_readlane(known, 16 * half), base + 16 * half) + head;
+            const char *from = reinterpret_cast<const char *>(array + at);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                got[4 * half + e] = __builtin_nontemporal_load(reinterpret_cast<const row_t *>(from + along[e]));
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int r = 16 * (e / 4) + 4 * (lane / 16) + e % 4;
+            const int64_t at = row_offset(p.cache, __shfl(known, r), base + r) + head + (DIM / 16) * (lane % 16);
+            got[e] = __builtin_nontemporal_load(reinterpret_cast<const row_t *>(array + at));
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+#pragma unroll
+        for (int i = 0; i < DIM / 32; ++i)
+            rows[e][i] = got[e][i];
+}
+
+// Where 16-byte chunk `chunk` of key row `row` lies in a wavefront's part of LDS: rows turned so that the
+// 16 rows of a fragment lie on different banks.
+template <int DIM> __device__ __forceinline__ int key_slot(int row, int chunk)
+{
+    constexpr int CHUNKS = DIM / 8;
+    return row * DIM + (chunk ^ (CHUNKS == 16 ? row & 15 : row >> 1 & 7)) * 8;
+}
+
+// Key rows as the lanes loaded them into a wavefront's own part of LDS, whose accesses stay in order without
+// a barrier.
 template <int DIM>
-__device__ __forceinline__ void load_tile(const DecodeParams &p, int base, int page, int query, size_t head, int lane,
-                                          Tile<DIM> &tile)
+__device__ __forceinline__ void park_keys(const unsigned (&rows)[8][DIM / 32], int lane, unsigned short *keys)
 {
     typedef unsigned row_t __attribute__((ext_vector_type(DIM / 32)));
     const int m = lane % 16, j = lane / 16;
-    const int position = base + lane % TILE;
-    tile.mask = unsigned(__ballot(page >= 0 && sees(p.see, query, position)));
-    const int known = page < 0 ? 0 : page; // (a masked row is read from some page that exists, and not used)
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-        const int64_t at = row_offset(p.cache, __shfl(known, 16 * t + m), base + 16 * t + m);
-        const unsigned short *from = p.cache.k + at + head + 8 * j;
-#pragma unroll
-        for (int s = 0; s < DIM / 32; ++s)
-            tile.k[t][s] = *reinterpret_cast<const bf16x8_t *>(from + 32 * s);
-    }
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        const int r = 16 * (e / 4) + 4 * j + e % 4;
-        const int64_t at = row_offset(p.cache, __shfl(known, r), base + r);
-        const row_t got = *reinterpret_cast<const row_t *>(p.cache.v + at + head + (DIM / 16) * m);
+        row_t k;
 #pragma unroll
         for (int i = 0; i < DIM / 32; ++i)
-            tile.v[e][i] = got[i];
+            k[i] = rows[e][i];
+        *reinterpret_cast<row_t *>(keys + key_slot<DIM>(16 * (e / 4) + 4 * j + e % 4, m * (DIM / 16) / 8) + m * (DIM / 16) % 8) = k;
     }
+    asm volatile("" ::: "memory");
 }
 
+// The weights of a tile's positions: register r of score[t] is position 16 t + 4 j + r, head m.
 template <int DIM>
-__device__ __forceinline__ void attend(const DecodeParams &p, Tile<DIM> &tile, const bf16x8_t (&q)[DIM / 32], int lane,
-                                       Running<DIM> &run)
+__device__ __forceinline__ bf16x8_t weigh(float scale, unsigned mask, const bf16x8_t (&q)[DIM / 32], int lane,
+                                          const unsigned short *keys, Running<DIM> &run)
 {
-    const int j = lane / 16;
-    if (tile.mask == 0)
-        return; // nothing of it is seen (uniform)
+    const int m = lane % 16, j = lane / 16;
     f32x4_t score[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
         score[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int s = 0; s < DIM / 32; ++s)
-            score[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(tile.k[t][s], q[s], score[t], 0, 0, 0);
-        score[t] *= p.scale;
+            score[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                *reinterpret_cast<const bf16x8_t *>(keys + key_slot<DIM>(16 * t + m, 4 * s + j)), q[s], score[t], 0, 0, 0);
+        score[t] *= scale;
     }
-    if (tile.mask != ~0u) { // (uniform)
+    asm volatile("" ::: "memory");
+    if (mask != ~0u) { // (uniform)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const bool seen = (tile.mask >> (16 * (e / 4) + 4 * j + e % 4)) & 1;
-            if (!seen)
-                score[e / 4][e % 4] = -INFINITY;
-            // (a weight of zero times what a hidden row may hold, NaN or infinity, would reach the output)
+        for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int i = 0; i < DIM / 32; ++i)
-                tile.v[e][i] = seen ? tile.v[e][i] : 0u;
-        }
+            for (int r = 0; r < 4; ++r)
+                score[t][r] = (mask >> (16 * t + 4 * j + r)) & 1 ? score[t][r] : -INFINITY;
     }
     float top = fmaxf(fmaxf(fmaxf(score[0][0], score[0][1]), fmaxf(score[0][2], score[0][3])),
                       fmaxf(fmaxf(score[1][0], score[1][1]), fmaxf(score[1][2], score[1][3])));
@@ -129,7 +152,7 @@ __device__ __forceinline__ void attend(const DecodeParams &p, Tile<DIM> &tile, c
         top = fmaxf(top, __shfl_xor(top, 16));
         top = fmaxf(top, __shfl_xor(top, 32));
         top = fmaxf(top, run.top);
-        const float factor = run.top == top ? 1.f : exp2f(run.top - top);
+        const float factor = run.top == top ? 1.f : __builtin_amdgcn_exp2f(run.top - top);
         run.top = top;
         run.total *= factor;
 #pragma unroll
@@ -148,36 +171,60 @@ __device__ __forceinline__ void attend(const DecodeParams &p, Tile<DIM> &tile, c
         weights[2 * t] = round_pair(score[t][0], score[t][1]);
         weights[2 * t + 1] = round_pair(score[t][2], score[t][3]);
     }
-    const bf16x8_t p_frag = __builtin_bit_cast(bf16x8_t, weights);
+    return __builtin_bit_cast(bf16x8_t, weights);
+}
+
+template <int DIM>
+__device__ __forceinline__ void add_values(unsigned mask, bf16x8_t weights, unsigned (&v)[8][DIM / 32], int lane, Running<DIM> &run)
+{
+    if (mask != ~0u) { // (uniform) a weight of zero times what a hidden row may hold, NaN or infinity, would reach the output
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const bool seen = (mask >> (16 * (e / 4) + 4 * (lane / 16) + e % 4)) & 1;
+#pragma unroll
+            for (int i = 0; i < DIM / 32; ++i)
+                v[e][i] = seen ? v[e][i] : 0u;
+        }
+    }
 #pragma unroll
     for (int i = 0; i < DIM / 32; ++i) {
         u32x4_t even, odd;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-            even[c] = __builtin_amdgcn_perm(tile.v[2 * c + 1][i], tile.v[2 * c][i], 0x05040100u);
-            odd[c] = __builtin_amdgcn_perm(tile.v[2 * c + 1][i], tile.v[2 * c][i], 0x07060302u);
+            even[c] = __builtin_amdgcn_perm(v[2 * c + 1][i], v[2 * c][i], 0x05040100u);
+            odd[c] = __builtin_amdgcn_perm(v[2 * c + 1][i], v[2 * c][i], 0x07060302u);
         }
-        run.acc[2 * i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, even), p_frag,
-                                                                  run.acc[2 * i], 0, 0, 0);
-        run.acc[2 * i + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, odd), p_frag,
-                                                                      run.acc[2 * i + 1], 0, 0, 0);
+        run.acc[2 * i] =
+            __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, even), weights, run.acc[2 * i], 0, 0, 0);
+        run.acc[2 * i + 1] =
+            __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, odd), weights, run.acc[2 * i + 1], 0, 0, 0);
     }
 }
 
-// slot < 0: this workgroup holds the whole of it and writes the output; otherwise partial `slot`
-template <int DIM>
-__device__ __forceinline__ void work_item(const DecodeParams &p, const Item &item, const TileSpan<TILE> &span, int query,
-                                          int first, int last, int slot)
+// page: those of the wavefront's first tile (fetch_page). slot < 0: this workgroup holds the whole of it and writes
+// the output; otherwise partial `slot`
+template <int DIM, bool LARGE>
+__device__ __forceinline__ void work_item(const DecodeParams &p, const unsigned short *queries, float scale, const Item item, const TileSpan<TILE> span, int query,
+                                          int first, int last, int page, int slot)
 {
-    __shared__ float wave_o[WAVES][HEADS][DIM + 4];
+    // (the outputs of the wavefronts, once they are done with their keys)
+    constexpr int KEYS = TILE * DIM * 2, OUTPUTS = HEADS * (DIM + 4) * 4;
+    __shared__ __attribute__((aligned(16))) unsigned char room[WAVES * (KEYS > OUTPUTS ? KEYS : OUTPUTS)];
+    float(*wave_o)[HEADS][DIM + 4] = reinterpret_cast<float(*)[HEADS][DIM + 4]>(room);
     __shared__ float wave_m[WAVES][HEADS], wave_l[WAVES][HEADS];
-    const int thread = threadIdx.x, lane = thread % 64, wave = thread / 64, m = lane % 16, j = lane / 16;
+    const int thread = threadIdx.x, lane = thread % 64, m = lane % 16, j = lane / 16;
+    const int wave = __builtin_amdgcn_readfirstlane(thread / 64);
+    unsigned short *keys = reinterpret_cast<unsigned short *>(room + wave * KEYS);
     const int32_t *row = p.table.pages + int64_t(item.sequence) * p.table.stride;
-    const size_t head_at = size_t(item.kv_head) * p.cache.head_stride;
+    const int64_t head_at = int64_t(item.kv_head) * p.cache.head_stride;
+    u32x4_t along;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        along[e] = LARGE ? (unsigned(4 * j + e) * unsigned(p.cache.slot_stride) + unsigned(DIM / 16 * m)) * 2 : 0;
     bf16x8_t q[DIM / 32];
     {
         const int head = item.head0 + (m < item.heads ? m : item.heads - 1);
-        const unsigned short *from = p.q + int64_t(item.sequence) * p.q_stride + int64_t(head) * DIM + 8 * j;
+        const unsigned short *from = queries + int64_t(item.sequence) * p.q_stride + int64_t(head) * DIM + 8 * j;
 #pragma unroll
         for (int s = 0; s < DIM / 32; ++s)
             q[s] = *reinterpret_cast<const bf16x8_t *>(from + 32 * s);
@@ -190,39 +237,37 @@ __device__ __forceinline__ void work_item(const DecodeParams &p, const Item &ite
         run.acc[w] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 
     const int end = min(last * WAVES, span.tiles);
+    __syncthreads(); // (outputs of the item before may still be read)
     int tile = __builtin_amdgcn_readfirstlane(first * WAVES + wave);
     if (tile < end) {
-        Tile<DIM> a, b;
+        // The next tile's keys are loaded as soon as this one's have gone to LDS, its values as soon as this one's
+        // are multiplied: one set of registers each, and one of the two always on its way.
+        unsigned k[8][DIM / 32], v[8][DIM / 32];
+        const auto seen = [&](int page, int base) { return unsigned(__ballot(page >= 0 && sees(p.see, query, base + lane % TILE))); };
         int base = span.position(tile);
-        int page = fetch_page<DIM>(p, row, base, lane);
-        load_tile<DIM>(p, base, page, query, head_at, lane, a);
-        tile += WAVES;
-        base = span.position(min(tile, span.tiles - 1));
-        page = fetch_page<DIM>(p, row, base, lane);
+        unsigned mask = seen(page, base);
+        load_rows<DIM, LARGE>(p, p.cache.k, base, page, head_at, lane, along, k);
+        load_rows<DIM, LARGE>(p, p.cache.v, base, page, head_at, lane, along, v);
+        base = span.position(min(tile + WAVES, span.tiles - 1));
+        page = fetch_page(p, row, base, lane);
         for (;;) {
-            // two tiles a turn, so that both sets of registers have fixed names: the next tile's rows travel
-            // while this one is worked on, and the page numbers of the one after that
+            tile += WAVES;
+            park_keys<DIM>(k, lane, keys);
             if (tile < end)
-                load_tile<DIM>(p, base, page, query, head_at, lane, b);
-            base = span.position(min(tile + WAVES, span.tiles - 1));
-            page = fetch_page<DIM>(p, row, base, lane);
-            attend<DIM>(p, a, q, lane, run);
+                load_rows<DIM, LARGE>(p, p.cache.k, base, page, head_at, lane, along, k);
+            const bf16x8_t weights = weigh<DIM>(scale, mask, q, lane, keys, run);
+            add_values<DIM>(mask, weights, v, lane, run);
             if (tile >= end)
                 break;
-            tile += WAVES;
-            if (tile < end)
-                load_tile<DIM>(p, base, page, query, head_at, lane, a);
+            mask = seen(page, base);
+            load_rows<DIM, LARGE>(p, p.cache.v, base, page, head_at, lane, along, v);
             base = span.position(min(tile + WAVES, span.tiles - 1));
-            page = fetch_page<DIM>(p, row, base, lane);
-            attend<DIM>(p, b, q, lane, run);
-            if (tile >= end)
-                break;
-            tile += WAVES;
+            page = fetch_page(p, row, base, lane);
         }
     }
     run.total += __shfl_xor(run.total, 16);
     run.total += __shfl_xor(run.total, 32);
-    __syncthreads(); // (the rows below may still be read for the item before)
+    __syncthreads(); // (keys of other wavefronts may still be read)
     if (j == 0) {
         wave_m[wave][m] = run.top;
         wave_l[wave][m] = run.total;
@@ -275,16 +320,32 @@ __device__ __forceinline__ Item item_of(const DecodeParams &p, int sequence, int
     return Item{sequence, kv_head, kv_head * p.group + first, min(HEADS, p.group - first)};
 }
 
-// one workgroup per (heads, sequence)
-template <int DIM> __global__ __launch_bounds__(WAVES * 64, 2) void paged_decode_whole_kernel(DecodeParams p)
+// The pages of the first tile a wavefront takes from step `first` on.
+__device__ __forceinline__ int first_page(const DecodeParams &p, const TileSpan<TILE> span, int sequence, int first)
 {
-    int query;
-    const TileSpan<TILE> span = span_of(p, blockIdx.y, query);
-    work_item<DIM>(p, item_of(p, blockIdx.y, blockIdx.x), span, query, 0, (span.tiles + WAVES - 1) / WAVES, -1);
+    const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x / 64)), lane = threadIdx.x % 64;
+    const int tile = first * WAVES + wave;
+    return tile < span.tiles
+               ? fetch_page(p, p.table.pages + int64_t(sequence) * p.table.stride, span.position(tile), lane) : -1;
+}
+
+// one workgroup per (heads, sequence)
+template <int DIM, bool LARGE> __global__ __launch_bounds__(WAVES * 64, 2) void paged_decode_whole_kernel(DecodeParams p)
+{
+    const int sequence = blockIdx.y;
+    int query, page = -1;
+    if (p.see.window <= 0) { // the pages travel together with the length that says whether they are needed
+        const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x / 64));
+        page = fetch_page(p, p.table.pages + int64_t(sequence) * p.table.stride, wave * TILE, threadIdx.x % 64);
+    }
+    const TileSpan<TILE> span = span_of(p, sequence, query);
+    if (p.see.window > 0)
+        page = first_page(p, span, sequence, 0);
+    work_item<DIM, LARGE>(p, p.q, p.scale, item_of(p, sequence, blockIdx.x), span, query, 0, (span.tiles + WAVES - 1) / WAVES, page, -1);
 }
 
 // every workgroup an equal run of all steps
-template <int DIM> __global__ __launch_bounds__(WAVES * 64, 2) void paged_decode_shares_kernel(DecodeParams p)
+template <int DIM, bool LARGE> __global__ __launch_bounds__(WAVES * 64, 2) void paged_decode_shares_kernel(DecodeParams p)
 {
     constexpr int THREADS = WAVES * 64;
     __shared__ int64_t wave_total[WAVES];
@@ -292,6 +353,8 @@ template <int DIM> __global__ __launch_bounds__(WAVES * 64, 2) void paged_decode
     __shared__ int found_sequence;
     const int thread = threadIdx.x, lane = thread % 64, wave = thread / 64;
     const int items = p.cache.kv_heads * p.head_tiles;
+    const unsigned short *queries = p.q;
+    const float scale = p.scale;
     // steps before each thread's run of sequences
     const int per = (p.batch + THREADS - 1) / THREADS;
     const int from = min(thread * per, p.batch), to = min(from + per, p.batch);
@@ -351,7 +414,8 @@ template <int DIM> __global__ __launch_bounds__(WAVES * 64, 2) void paged_decode
                 const int64_t ends = ((begins + steps) * workers - 1) / all;
                 p.joins[size_t(sequence) * items + index] = int2{int(blockIdx.x), int(ends)};
             }
-            work_item<DIM>(p, item_of(p, sequence, index), span, query, first, last, slot);
+            work_item<DIM, LARGE>(p, queries, scale, item_of(p, sequence, index), span, query, first, last,
+                                  first_page(p, span, sequence, first), slot);
             step = begins + last;
         }
         start += int64_t(steps) * items;
@@ -429,12 +493,17 @@ template <int DIM> __global__ __launch_bounds__(JOIN_THREADS) void paged_decode_
 } // namespace
 
 // How a call is divided: workgroups that share all steps, or 0 for one workgroup per (heads, sequence).
+// Sharing costs a second launch and the numbering of the steps, some 6 us, and keeps every compute unit busy
+// whatever the lengths; one workgroup each is done when the longest sequence is. Measured, 64 query and 8
+// key-value heads of 128, whole / shared: 8 items of 512 positions 11.7 / 12.3 us, of 1024 18 / 12; 128 items of
+// 1024 20 / 21, of 2048 35 / 32 (lengths from 1 to that 30 / 21); 256 items of 2048 46 / 53 (36 / 38), of 4096
+// 85 / 93 (64 / 52).
 static int decode_shares(int64_t items, int64_t positions, int compute_units)
 {
-    const int64_t shares = 2 * compute_units < MOST_SHARES ? 2 * compute_units : MOST_SHARES;
-    if (positions <= 512 || items >= 4 * shares)
+    const int64_t busy = items < compute_units ? items : compute_units;
+    if (positions <= 512 + 1792 * busy / compute_units)
         return 0;
-    return int(shares);
+    return 2 * compute_units < MOST_SHARES ? 2 * compute_units : MOST_SHARES;
 }
 
 static int64_t decode_positions(int64_t capacity, const Visibility &see)
@@ -470,12 +539,13 @@ hipError_t launch_paged_decode(hipStream_t stream, int batch, int q_heads, int d
     p.out = static_cast<unsigned short *>(out);
     p.q_stride = q_stride;
     p.out_stride = out_stride;
+    // (16 rows within the reach of 32-bit offsets)
+    const bool large = cache.page_shift >= 4 && cache.slot_stride < (int64_t(1) << 26);
     if (shares == 0) {
         const dim3 grid(items, batch);
-        if (dim == 128)
-            paged_decode_whole_kernel<128><<<grid, WAVES * 64, 0, stream>>>(p);
-        else
-            paged_decode_whole_kernel<64><<<grid, WAVES * 64, 0, stream>>>(p);
+        const auto kernel = dim == 128 ? (large ? paged_decode_whole_kernel<128, true> : paged_decode_whole_kernel<128, false>)
+                                       : (large ? paged_decode_whole_kernel<64, true> : paged_decode_whole_kernel<64, false>);
+        kernel<<<grid, WAVES * 64, 0, stream>>>(p);
         return launch_status();
     }
     const size_t rows = 2 * size_t(shares) * HEADS;
@@ -483,10 +553,9 @@ hipError_t launch_paged_decode(hipStream_t stream, int batch, int q_heads, int d
     p.part_m = p.part_o + rows * dim;
     p.part_l = p.part_m + rows;
     p.joins = reinterpret_cast<int2 *>(p.part_l + rows);
-    if (dim == 128)
-        paged_decode_shares_kernel<128><<<shares, WAVES * 64, 0, stream>>>(p);
-    else
-        paged_decode_shares_kernel<64><<<shares, WAVES * 64, 0, stream>>>(p);
+    const auto kernel = dim == 128 ? (large ? paged_decode_shares_kernel<128, true> : paged_decode_shares_kernel<128, false>)
+                                   : (large ? paged_decode_shares_kernel<64, true> : paged_decode_shares_kernel<64, false>);
+    kernel<<<shares, WAVES * 64, 0, stream>>>(p);
     hipError_t status = launch_status();
     if (status != hipSuccess)
         return status;
