@@ -103,7 +103,8 @@ SIGNATURES = {
     "qk_norm_rope_append": ([_P, _I, _I, _I, _F, _I, _F, _P, _P, _P, _P, _P, _L, _P, _L, _P], _I),
     "paged_decode_workspace_size": ([_P, _I, _I, _P, _I, _I, _I], _SZ),
     "paged_decode_attention": ([_P, _I, _I, _P, _P, _L, _I, _P, _I, _I, _F, _P, _L, _P, _SZ, _P, _L], _I),
-    "paged_prefill_attention": ([_P, _I, _I, _I, _P, _P, _L, _I, _P, _P, _I, _I, _F, _P, _L, _P, _L], _I),
+    "paged_prefill_workspace_size": ([_P, _I, _I, _I, _P, _I, _I, _I], _SZ),
+    "paged_prefill_attention": ([_P, _I, _I, _I, _P, _P, _L, _I, _P, _P, _I, _I, _F, _P, _L, _P, _SZ, _P, _L], _I),
     "hip_plan_describe": ([_I, _I, _C, _C, _I, _I, _I, _I, _I, _I, _I, ct.c_char_p, _SZ], _I),
     "hip_set_plan_override": ([_P, _I, _I], _I),
     "hip_kernel_count": ([_I], _I),

@@ -138,11 +138,24 @@ extern "C" int camblas_cuda_paged_decode_attention(camblas_cuda_context *context
     });
 }
 
+extern "C" size_t camblas_cuda_paged_prefill_workspace_size(const camblas_cuda_context *context, int batch, int tokens,
+                                                            int q_heads, const camblas_cuda_paged_cache *cache,
+                                                            int table_columns, int window, int sinks)
+{
+    if (!context || !valid_cache(cache) ||
+        !valid_attention(batch, tokens, q_heads, cache, table_columns, table_columns, window, sinks, 1.f,
+                         int64_t(q_heads) * cache->dim, int64_t(q_heads) * cache->dim))
+        return 0;
+    return paged_prefill_workspace(batch, tokens, q_heads, cache->kv_heads, cache->dim,
+                                   int64_t(table_columns) * cache->page_size, window, sinks, context->compute_units);
+}
+
 extern "C" int camblas_cuda_paged_prefill_attention(camblas_cuda_context *context, int batch, int tokens, int q_heads,
                                                     const camblas_cuda_paged_cache *cache, const int32_t *page_table,
                                                     int64_t table_stride, int table_columns, const int32_t *lengths,
                                                     const int32_t *query_starts, int window, int sinks, float scale,
-                                                    const void *q, int64_t q_stride, void *output, int64_t output_stride)
+                                                    const void *q, int64_t q_stride, void *workspace,
+                                                    size_t workspace_bytes, void *output, int64_t output_stride)
 {
     Entry entry(context);
     return entry.run([&] {
@@ -156,11 +169,16 @@ extern "C" int camblas_cuda_paged_prefill_attention(camblas_cuda_context *contex
         if (!usable({{page_table, 4, table_columns == 0}, {lengths, 4}, {query_starts, 4}, {q, 16}, {output, 16}}) ||
             !apart(output, {q, cache->k, cache->v, page_table, lengths, query_starts}))
             return entry.refuse("invalid paged attention buffers");
+        const size_t bytes = paged_prefill_workspace(batch, tokens, q_heads, cache->kv_heads, cache->dim,
+                                                     int64_t(table_columns) * cache->page_size, window, sinks,
+                                                     context->compute_units);
+        if (bytes && (!usable({{workspace, 16}}) || workspace_bytes < bytes))
+            return entry.refuse("paged attention workspace is missing, misaligned or too small");
         context->counts[6]++;
         return entry.finish(launch_paged_prefill(entry.stream(), batch, tokens, q_heads, cache->dim, device_cache(cache),
                                                  PageTable{page_table, lengths, table_stride, table_columns},
                                                  Visibility{window, sinks}, query_starts, scale, q, q_stride, output,
-                                                 output_stride, context->compute_units),
+                                                 output_stride, workspace, context->compute_units),
                             "paged prefill attention");
     });
 }

@@ -160,10 +160,16 @@ Tensor prefill(const Tensor &q, const Tensor &k_cache, const Tensor &v_cache, co
     Attention a(q, k_cache, v_cache, page_table, lengths, scale, window, sinks, out);
     check_integers("query_starts", query_starts, at::kInt, int64_t(a.batch) + 1, a.device);
     camblas_cuda_context *context = context_for(a.device.index(), current_default_algorithm());
+    const size_t bytes =
+        camblas_cuda_paged_prefill_workspace_size(context, a.batch, a.tokens, a.q_heads, &a.cache, a.columns, a.window, a.sinks);
+    Tensor workspace;
+    if (bytes)
+        workspace = at::empty({int64_t(bytes)}, q.options().dtype(at::kByte));
     succeed(camblas_cuda_paged_prefill_attention(
                 context, a.batch, a.tokens, a.q_heads, &a.cache, page_table.const_data_ptr<int32_t>(), page_table.stride(0),
                 a.columns, lengths.const_data_ptr<int32_t>(), query_starts.const_data_ptr<int32_t>(), a.window, a.sinks,
-                a.scale, q.const_data_ptr(), a.q_stride, a.output.mutable_data_ptr(), a.output_stride),
+                a.scale, q.const_data_ptr(), a.q_stride, bytes ? workspace.mutable_data_ptr() : nullptr, bytes,
+                a.output.mutable_data_ptr(), a.output_stride),
             context);
     return a.output;
 }

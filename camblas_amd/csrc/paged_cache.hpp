@@ -39,9 +39,12 @@ size_t paged_decode_workspace(int batch, int q_heads, int kv_heads, int dim, int
 hipError_t launch_paged_decode(hipStream_t stream, int batch, int q_heads, int dim, const PagedCache &cache,
                                const PageTable &table, const Visibility &see, float scale, const void *q,
                                int64_t q_stride, void *out, int64_t out_stride, void *workspace, int compute_units);
+size_t paged_prefill_workspace(int batch, int tokens, int q_heads, int kv_heads, int dim, int64_t capacity, int window, int sinks,
+                               int compute_units);
 hipError_t launch_paged_prefill(hipStream_t stream, int batch, int tokens, int q_heads, int dim, const PagedCache &cache,
                                 const PageTable &table, const Visibility &see, const int32_t *starts, float scale,
-                                const void *q, int64_t q_stride, void *out, int64_t out_stride, int compute_units);
+                                const void *q, int64_t q_stride, void *out, int64_t out_stride, void *workspace,
+                                int compute_units);
 
 // Two values to BF16 in one word, round to nearest even, NaN stays NaN: one instruction.
 __device__ __forceinline__ unsigned round_pair(float lo, float hi)

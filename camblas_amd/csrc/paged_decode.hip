@@ -27,7 +27,7 @@ namespace camblas_hip
 {
 namespace
 {
-constexpr int WAVES = 4, TILE = 32, HEADS = 16, JOIN_THREADS = 256, MOST_SHARES = 1024;
+constexpr int TILE = 32, HEADS = 16, JOIN_THREADS = 256, MOST_SHARES = 1024, SHARE_WAVES = 4;
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct DecodeParams {
@@ -203,7 +203,7 @@ __device__ __forceinline__ void add_values(unsigned mask, bf16x8_t weights, unsi
 
 // page: those of the wavefront's first tile (fetch_page). slot < 0: this workgroup holds the whole of it and writes
 // the output; otherwise partial `slot`
-template <int DIM, bool LARGE>
+template <int DIM, bool LARGE, int WAVES>
 __device__ __forceinline__ void work_item(const DecodeParams &p, const unsigned short *queries, float scale, const Item item, const TileSpan<TILE> span, int query,
                                           int first, int last, int page, int slot)
 {
@@ -321,6 +321,7 @@ __device__ __forceinline__ Item item_of(const DecodeParams &p, int sequence, int
 }
 
 // The pages of the first tile a wavefront takes from step `first` on.
+template <int WAVES>
 __device__ __forceinline__ int first_page(const DecodeParams &p, const TileSpan<TILE> span, int sequence, int first)
 {
     const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x / 64)), lane = threadIdx.x % 64;
@@ -330,7 +331,7 @@ __device__ __forceinline__ int first_page(const DecodeParams &p, const TileSpan<
 }
 
 // one workgroup per (heads, sequence)
-template <int DIM, bool LARGE> __global__ __launch_bounds__(WAVES * 64, 2) void paged_decode_whole_kernel(DecodeParams p)
+template <int DIM, bool LARGE, int WAVES> __global__ __launch_bounds__(WAVES * 64, 2) void paged_decode_whole_kernel(DecodeParams p)
 {
     const int sequence = blockIdx.y;
     int query, page = -1;
@@ -340,14 +341,14 @@ template <int DIM, bool LARGE> __global__ __launch_bounds__(WAVES * 64, 2) void 
     }
     const TileSpan<TILE> span = span_of(p, sequence, query);
     if (p.see.window > 0)
-        page = first_page(p, span, sequence, 0);
-    work_item<DIM, LARGE>(p, p.q, p.scale, item_of(p, sequence, blockIdx.x), span, query, 0, (span.tiles + WAVES - 1) / WAVES, page, -1);
+        page = first_page<WAVES>(p, span, sequence, 0);
+    work_item<DIM, LARGE, WAVES>(p, p.q, p.scale, item_of(p, sequence, blockIdx.x), span, query, 0, (span.tiles + WAVES - 1) / WAVES, page, -1);
 }
 
 // every workgroup an equal run of all steps
-template <int DIM, bool LARGE> __global__ __launch_bounds__(WAVES * 64, 2) void paged_decode_shares_kernel(DecodeParams p)
+template <int DIM, bool LARGE> __global__ __launch_bounds__(SHARE_WAVES * 64, 2) void paged_decode_shares_kernel(DecodeParams p)
 {
-    constexpr int THREADS = WAVES * 64;
+    constexpr int WAVES = SHARE_WAVES, THREADS = WAVES * 64;
     __shared__ int64_t wave_total[WAVES];
     __shared__ int64_t found_start;
     __shared__ int found_sequence;
@@ -414,8 +415,8 @@ template <int DIM, bool LARGE> __global__ __launch_bounds__(WAVES * 64, 2) void 
                 const int64_t ends = ((begins + steps) * workers - 1) / all;
                 p.joins[size_t(sequence) * items + index] = int2{int(blockIdx.x), int(ends)};
             }
-            work_item<DIM, LARGE>(p, queries, scale, item_of(p, sequence, index), span, query, first, last,
-                                  first_page(p, span, sequence, first), slot);
+            work_item<DIM, LARGE, WAVES>(p, queries, scale, item_of(p, sequence, index), span, query, first, last,
+                                  first_page<WAVES>(p, span, sequence, first), slot);
             step = begins + last;
         }
         start += int64_t(steps) * items;
@@ -519,6 +520,15 @@ size_t paged_decode_workspace(int batch, int q_heads, int kv_heads, int dim, int
     return shares ? 2 * shares * HEADS * (size_t(dim) + 2) * sizeof(float) + size_t(items) * sizeof(int2) : 0;
 }
 
+template <int WAVES>
+static void launch_whole(hipStream_t stream, int dim, bool large, dim3 grid, const DecodeParams &p)
+{
+    const auto kernel =
+        dim == 128 ? (large ? paged_decode_whole_kernel<128, true, WAVES> : paged_decode_whole_kernel<128, false, WAVES>)
+                   : (large ? paged_decode_whole_kernel<64, true, WAVES> : paged_decode_whole_kernel<64, false, WAVES>);
+    kernel<<<grid, WAVES * 64, 0, stream>>>(p);
+}
+
 hipError_t launch_paged_decode(hipStream_t stream, int batch, int q_heads, int dim, const PagedCache &cache,
                                const PageTable &table, const Visibility &see, float scale, const void *q,
                                int64_t q_stride, void *out, int64_t out_stride, void *workspace, int compute_units)
@@ -543,9 +553,11 @@ hipError_t launch_paged_decode(hipStream_t stream, int batch, int q_heads, int d
     const bool large = cache.page_shift >= 4 && cache.slot_stride < (int64_t(1) << 26);
     if (shares == 0) {
         const dim3 grid(items, batch);
-        const auto kernel = dim == 128 ? (large ? paged_decode_whole_kernel<128, true> : paged_decode_whole_kernel<128, false>)
-                                       : (large ? paged_decode_whole_kernel<64, true> : paged_decode_whole_kernel<64, false>);
-        kernel<<<grid, WAVES * 64, 0, stream>>>(p);
+        // (with less than a workgroup per compute unit eight wavefronts each: 8 items of 129 positions 8.0 / 7.3 us)
+        if (int64_t(batch) * items < compute_units)
+            launch_whole<8>(stream, dim, large, grid, p);
+        else
+            launch_whole<4>(stream, dim, large, grid, p);
         return launch_status();
     }
     const size_t rows = 2 * size_t(shares) * HEADS;
@@ -555,7 +567,7 @@ hipError_t launch_paged_decode(hipStream_t stream, int batch, int q_heads, int d
     p.joins = reinterpret_cast<int2 *>(p.part_l + rows);
     const auto kernel = dim == 128 ? (large ? paged_decode_shares_kernel<128, true> : paged_decode_shares_kernel<128, false>)
                                    : (large ? paged_decode_shares_kernel<64, true> : paged_decode_shares_kernel<64, false>);
-    kernel<<<shares, WAVES * 64, 0, stream>>>(p);
+    kernel<<<shares, SHARE_WAVES * 64, 0, stream>>>(p);
     hipError_t status = launch_status();
     if (status != hipSuccess)
         return status;

@@ -27,7 +27,7 @@ namespace camblas_hip
 {
 namespace
 {
-constexpr int WAVES = 4, THREADS = WAVES * 64, ROWS = WAVES * 32, TILE = 64;
+constexpr int WAVES = 4, THREADS = WAVES * 64, ROWS = WAVES * 32, TILE = 64, JOIN_ROWS = 32, MOST_SHARES = 32;
 constexpr int VECTOR = 0x2, MATRIX = 0x8, DS_READS = 0x100; // kinds of instructions for the scheduler
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -41,6 +41,9 @@ struct PrefillParams {
     const unsigned short *q;
     unsigned short *out;
     int64_t q_stride, out_stride;
+    // where positions are divided over `shares` workgroups per block of rows: [share][token][query head][dim], [..][..][..]
+    int shares;
+    float *part_o, *part_m, *part_l;
 };
 
 typedef short i16x4_t __attribute__((ext_vector_type(4)));
@@ -117,37 +120,52 @@ __device__ __forceinline__ int first_token(const PrefillParams &p, int sequence)
     return min(max(p.starts[sequence], 0), p.tokens);
 }
 
-template <int DIM> __global__ __launch_bounds__(THREADS, DIM == 64 ? 3 : 2) void paged_prefill_kernel(PrefillParams p)
+// A block of ROWS rows of one key-value head: row r of it is query head r % group of token r / group.
+struct Block {
+    int sequence, kv_head, token0, tokens; // the sequence's first token and how many it has
+    int64_t row0, rows;                    // the block's first row, how many rows the sequence has from there on
+};
+
+// Blocks of sequence b are numbered from floor(first token * group / ROWS) + b: a number that needs no
+// sum over the sequences before, leaves room for a last block that is not full, and at most one unused
+// number per sequence. False for an unused number.
+__device__ __forceinline__ bool find_block(const PrefillParams &p, int number, Block &block)
+{
+    __shared__ int found;
+    // the last blocks of a causal sequence see most: they start first
+    block.kv_head = number % p.cache.kv_heads;
+    const int wanted = p.row_blocks - 1 - number / p.cache.kv_heads;
+    if (threadIdx.x == 0)
+        found = 0;
+    __syncthreads();
+    for (int b = threadIdx.x; b < p.batch; b += THREADS) {
+        const int64_t here = int64_t(first_token(p, b)) * p.group / ROWS + b;
+        const int64_t next = int64_t(first_token(p, b + 1)) * p.group / ROWS + b + 1;
+        if (here <= wanted && wanted < next)
+            found = b;
+    }
+    __syncthreads();
+    block.sequence = uniform(found);
+    block.token0 = uniform(first_token(p, block.sequence));
+    block.tokens = uniform(first_token(p, block.sequence + 1)) - block.token0;
+    block.row0 = (wanted - (int64_t(block.token0) * p.group / ROWS + block.sequence)) * ROWS;
+    block.rows = int64_t(block.tokens) * p.group - block.row0;
+    return block.row0 >= 0 && block.rows > 0;
+}
+
+// SHARED: blockIdx.y of `shares` workgroups takes its part of the tiles and leaves what it has for the join.
+template <int DIM, bool SHARED> __global__ __launch_bounds__(THREADS, DIM == 64 ? 3 : 2) void paged_prefill_kernel(PrefillParams p)
 {
     constexpr int CHUNKS = DIM / 8, FETCH = 64 / CHUNKS, FETCHES = TILE / FETCH / WAVES; // rows of a load, a wavefront's loads
     __shared__ __attribute__((aligned(16))) unsigned char keys0[TILE * DIM * 2], keys1[TILE * DIM * 2];
     __shared__ __attribute__((aligned(16))) unsigned char values0[TILE * DIM * 2], values1[TILE * DIM * 2];
-    __shared__ int found;
     const int thread = threadIdx.x, lane = thread % 64, wave = uniform(thread / 64);
     const int column = lane % 32, half = lane / 32;
-    // the last blocks of a causal sequence see most: they start first
-    const int kv_head = int(blockIdx.x) % p.cache.kv_heads;
-    const int block = p.row_blocks - 1 - int(blockIdx.x) / p.cache.kv_heads;
-
-    // Blocks of sequence b are numbered from floor(first token * group / ROWS) + b: a number that needs no
-    // sum over the sequences before, leaves room for a last block that is not full, and at most one unused
-    // number per sequence.
-    if (thread == 0)
-        found = 0;
-    __syncthreads();
-    for (int b = thread; b < p.batch; b += THREADS) {
-        const int64_t here = int64_t(first_token(p, b)) * p.group / ROWS + b;
-        const int64_t next = int64_t(first_token(p, b + 1)) * p.group / ROWS + b + 1;
-        if (here <= block && block < next)
-            found = b;
-    }
-    __syncthreads();
-    const int sequence = __builtin_amdgcn_readfirstlane(found);
-    const int token0 = uniform(first_token(p, sequence)), tokens = uniform(first_token(p, sequence + 1)) - token0;
-    const int64_t row0 = (block - (int64_t(token0) * p.group / ROWS + sequence)) * ROWS;
-    const int64_t rows = int64_t(tokens) * p.group - row0;
-    if (row0 < 0 || rows <= 0)
+    Block block;
+    if (!find_block(p, blockIdx.x, block))
         return;
+    const int sequence = block.sequence, kv_head = block.kv_head, token0 = block.token0, tokens = block.tokens;
+    const int64_t row0 = block.row0, rows = block.rows;
 
     // ---- this lane's row: token and query head, position
     const int past = uniform(live_positions(p.table, p.cache, sequence)) - tokens;
@@ -166,11 +184,13 @@ template <int DIM> __global__ __launch_bounds__(THREADS, DIM == 64 ? 3 : 2) void
     const int first_query = uniform(past + int(row0 / p.group));
     const int last_query = uniform(past + int((row0 + min(rows, int64_t(ROWS)) - 1) / p.group));
     const TileSpan<TILE> span(p.see, first_query, last_query);
+    const int first = SHARED ? int(int64_t(span.tiles) * blockIdx.y / p.shares) : 0;
+    const int end = SHARED ? int(int64_t(span.tiles) * (blockIdx.y + 1) / p.shares) : span.tiles;
 
     // ---- fetching tiles: lane r of every wavefront knows the page of tile row r
     const int32_t *pages = p.table.pages + int64_t(sequence) * p.table.stride;
     const auto page_at = [&](int tile) {
-        return tile < span.tiles ? page_of(p.cache, pages, p.table.columns, span.position(tile) + lane) : -1;
+        return tile < end ? page_of(p.cache, pages, p.table.columns, span.position(tile) + lane) : -1;
     };
     // which rows of a tile exist and are seen by some query of the block
     const auto wanted_rows = [&](int tile, int page) {
@@ -254,10 +274,10 @@ template <int DIM> __global__ __launch_bounds__(THREADS, DIM == 64 ? 3 : 2) void
                           const unsigned char *next_keys, unsigned char *values, unsigned char *next_values) {
         const int base = span.position(tile);
         const uint64_t next_wanted = wanted_rows(tile + 1, page);
-        if (tile + 1 < span.tiles)
+        if (tile + 1 < end)
             fetch(p.cache.v, value_from, at, tile + 1, page, next_values);
         page = next_page;
-        if (tile + 2 < span.tiles) {
+        if (tile + 2 < end) {
             at = place(tile + 2, page);
             fetch(p.cache.k, key_from, at, tile + 2, page, keys);
         }
@@ -351,17 +371,17 @@ template <int DIM> __global__ __launch_bounds__(THREADS, DIM == 64 ? 3 : 2) void
         asm volatile("" ::: "memory");
     };
 
-    if (span.tiles > 0) {
-        page = page_at(0);
-        wanted = wanted_rows(0, page);
-        at = place(0, page);
-        fetch(p.cache.k, key_from, at, 0, page, keys0);
-        fetch(p.cache.v, value_from, at, 0, page, values0);
-        page = page_at(1);
-        next_page = page_at(2);
-        if (span.tiles > 1) {
-            at = place(1, page);
-            fetch(p.cache.k, key_from, at, 1, page, keys1);
+    if (first < end) {
+        page = page_at(first);
+        wanted = wanted_rows(first, page);
+        at = place(first, page);
+        fetch(p.cache.k, key_from, at, first, page, keys0);
+        fetch(p.cache.v, value_from, at, first, page, values0);
+        page = page_at(first + 1);
+        next_page = page_at(first + 2);
+        if (first + 1 < end) {
+            at = place(first + 1, page);
+            fetch(p.cache.k, key_from, at, first + 1, page, keys1);
         }
         pipeline_barrier<0>();
         asm volatile("" ::: "memory");
@@ -370,9 +390,9 @@ template <int DIM> __global__ __launch_bounds__(THREADS, DIM == 64 ? 3 : 2) void
         asm volatile("" ::: "memory");
         pipeline_barrier<0>();
         asm volatile("" ::: "memory");
-        for (int tile = 0; tile < span.tiles; tile += 2) {
+        for (int tile = first; tile < end; tile += 2) {
             turn(tile, even, odd, keys0, keys1, values0, values1);
-            if (tile + 1 >= span.tiles)
+            if (tile + 1 >= end)
                 break;
             turn(tile + 1, odd, even, keys1, keys0, values1, values0);
         }
@@ -382,31 +402,109 @@ template <int DIM> __global__ __launch_bounds__(THREADS, DIM == 64 ? 3 : 2) void
     const float sum = total + __shfl_xor(total, 32);
     if (row >= row0 + rows)
         return;
-    // (no position seen: zero; a sum that is NaN stays NaN)
-    const float inverse = sum == 0.f ? 0.f : 1.f / sum;
     const int token = token0 + int(row / p.group), head = kv_head * p.group + int(row % p.group);
-    unsigned short *to = p.out + int64_t(token) * p.out_stride + int64_t(head) * DIM + 4 * half;
+    if constexpr (SHARED) {
+        const size_t at_row = (size_t(blockIdx.y) * p.tokens + token) * (p.cache.kv_heads * p.group) + head;
+        if (half == 0) {
+            p.part_m[at_row] = top;
+            p.part_l[at_row] = sum;
+        }
+        float *to = p.part_o + at_row * DIM + 4 * half;
 #pragma unroll
-    for (int d = 0; d < DIM / 32; ++d)
+        for (int d = 0; d < DIM / 32; ++d)
 #pragma unroll
-        for (int g = 0; g < 4; ++g)
-            *reinterpret_cast<u32x2_t *>(to + 32 * d + 8 * g) =
-                u32x2_t{round_pair(acc[d][4 * g] * inverse, acc[d][4 * g + 1] * inverse),
-                        round_pair(acc[d][4 * g + 2] * inverse, acc[d][4 * g + 3] * inverse)};
+            for (int g = 0; g < 4; ++g)
+                *reinterpret_cast<f32x4_t *>(to + 32 * d + 8 * g) =
+                    f32x4_t{acc[d][4 * g], acc[d][4 * g + 1], acc[d][4 * g + 2], acc[d][4 * g + 3]};
+    } else {
+        // (no position seen: zero; a sum that is NaN stays NaN)
+        const float inverse = sum == 0.f ? 0.f : 1.f / sum;
+        unsigned short *to = p.out + int64_t(token) * p.out_stride + int64_t(head) * DIM + 4 * half;
+#pragma unroll
+        for (int d = 0; d < DIM / 32; ++d)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                *reinterpret_cast<u32x2_t *>(to + 32 * d + 8 * g) =
+                    u32x2_t{round_pair(acc[d][4 * g] * inverse, acc[d][4 * g + 1] * inverse),
+                            round_pair(acc[d][4 * g + 2] * inverse, acc[d][4 * g + 3] * inverse)};
+    }
+}
+
+// Joins the shares of the rows of a block, JOIN_ROWS of them a workgroup, in their order; DIM / 4 threads take a row.
+template <int DIM> __global__ __launch_bounds__(THREADS) void paged_prefill_join_kernel(PrefillParams p)
+{
+    constexpr int ROW = DIM / 4;
+    Block block;
+    if (!find_block(p, blockIdx.x, block))
+        return;
+    const int d = 4 * (threadIdx.x % ROW), q_heads = p.cache.kv_heads * p.group;
+    const int64_t low = int64_t(blockIdx.y) * JOIN_ROWS, high = min(block.rows, low + JOIN_ROWS);
+    for (int64_t r = low + threadIdx.x / ROW; r < high; r += THREADS / ROW) {
+        const int64_t row = block.row0 + r;
+        const int token = block.token0 + int(row / p.group), head = block.kv_head * p.group + int(row % p.group);
+        const size_t first = size_t(token) * q_heads + head, step = size_t(p.tokens) * q_heads;
+        float top = -INFINITY;
+#pragma unroll 4
+        for (int s = 0; s < p.shares; ++s)
+            top = fmaxf(top, p.part_m[first + s * step]);
+        const float reference = top == -INFINITY ? 0.f : top;
+        f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+        float sum = 0.f;
+#pragma unroll 4
+        for (int s = 0; s < p.shares; ++s) {
+            const float factor = __builtin_amdgcn_exp2f(p.part_m[first + s * step] - reference);
+            sum = fmaf(factor, p.part_l[first + s * step], sum);
+            o += factor * *reinterpret_cast<const f32x4_t *>(p.part_o + (first + s * step) * DIM + d);
+        }
+        o *= sum == 0.f ? 0.f : 1.f / sum;
+        *reinterpret_cast<u32x2_t *>(p.out + int64_t(token) * p.out_stride + int64_t(head) * DIM + d) =
+            u32x2_t{round_pair(o[0], o[1]), round_pair(o[2], o[3])};
+    }
+}
+
+int64_t prefill_blocks(int batch, int tokens, int group) { return int64_t(tokens) * group / ROWS + batch; }
+
+// Over how many workgroups the positions of a block of rows are divided: as many as fill the chip where the
+// blocks alone do not, with a few tiles each.
+int prefill_shares(int64_t blocks, int dim, int64_t positions, int compute_units)
+{
+    const int64_t room = int64_t(dim == 64 ? 3 : 2) * compute_units / (blocks > 0 ? blocks : 1);
+    const int64_t enough = positions / (4 * TILE);
+    const int64_t shares = room < enough ? room : enough;
+    return shares < 2 ? 1 : shares < MOST_SHARES ? int(shares) : MOST_SHARES;
+}
+
+// the most positions that a block of rows can see
+int64_t prefill_positions(int64_t capacity, const Visibility &see, int tokens, int group)
+{
+    const int64_t reach = int64_t(see.window) + see.sinks + (tokens < ROWS / group + 1 ? tokens : ROWS / group + 1);
+    return see.window > 0 && reach < capacity ? reach : capacity;
 }
 } // namespace
 
+size_t paged_prefill_workspace(int batch, int tokens, int q_heads, int kv_heads, int dim, int64_t capacity, int window, int sinks,
+                               int compute_units)
+{
+    const int group = q_heads / kv_heads;
+    const int shares = prefill_shares(prefill_blocks(batch, tokens, group) * kv_heads, dim,
+                                      prefill_positions(capacity, Visibility{window, sinks}, tokens, group), compute_units);
+    return shares > 1 ? size_t(shares) * tokens * q_heads * (size_t(dim) + 2) * sizeof(float) : 0;
+}
+
 hipError_t launch_paged_prefill(hipStream_t stream, int batch, int tokens, int q_heads, int dim, const PagedCache &cache,
                                 const PageTable &table, const Visibility &see, const int32_t *starts, float scale,
-                                const void *q, int64_t q_stride, void *out, int64_t out_stride, int compute_units)
+                                const void *q, int64_t q_stride, void *out, int64_t out_stride, void *workspace,
+                                int compute_units)
 {
     PrefillParams p = {};
     p.batch = batch;
     p.tokens = tokens;
     p.group = q_heads / cache.kv_heads;
-    const int64_t blocks = int64_t(tokens) * p.group / ROWS + batch;
+    const int64_t blocks = prefill_blocks(batch, tokens, p.group);
     if (blocks * cache.kv_heads > INT32_MAX)
         return hipErrorInvalidValue;
+    const int64_t capacity = int64_t(table.columns) << cache.page_shift;
+    p.shares = prefill_shares(blocks * cache.kv_heads, dim, prefill_positions(capacity, see, tokens, p.group), compute_units);
     p.row_blocks = int(blocks);
     p.cache = cache;
     p.table = table;
@@ -417,11 +515,23 @@ hipError_t launch_paged_prefill(hipStream_t stream, int batch, int tokens, int q
     p.out = static_cast<unsigned short *>(out);
     p.q_stride = q_stride;
     p.out_stride = out_stride;
-    const unsigned grid = unsigned(blocks * cache.kv_heads);
-    if (dim == 128)
-        paged_prefill_kernel<128><<<grid, WAVES * 64, 0, stream>>>(p);
-    else
-        paged_prefill_kernel<64><<<grid, WAVES * 64, 0, stream>>>(p);
+    const unsigned numbers = unsigned(blocks * cache.kv_heads);
+    if (p.shares == 1) {
+        const auto kernel = dim == 128 ? paged_prefill_kernel<128, false> : paged_prefill_kernel<64, false>;
+        kernel<<<numbers, THREADS, 0, stream>>>(p);
+        return launch_status();
+    }
+    const size_t rows = size_t(p.shares) * tokens * q_heads;
+    p.part_o = static_cast<float *>(workspace);
+    p.part_m = p.part_o + rows * dim;
+    p.part_l = p.part_m + rows;
+    const auto kernel = dim == 128 ? paged_prefill_kernel<128, true> : paged_prefill_kernel<64, true>;
+    kernel<<<dim3(numbers, p.shares), THREADS, 0, stream>>>(p);
+    const hipError_t status = launch_status();
+    if (status != hipSuccess)
+        return status;
+    const auto join = dim == 128 ? paged_prefill_join_kernel<128> : paged_prefill_join_kernel<64>;
+    join<<<dim3(numbers, ROWS / JOIN_ROWS), THREADS, 0, stream>>>(p);
     return launch_status();
 }
 } // namespace camblas_hip

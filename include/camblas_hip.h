@@ -434,15 +434,19 @@ int camblas_cuda_paged_decode_attention(camblas_cuda_context *context, int batch
                                         int64_t table_stride, int table_columns, const int32_t *lengths, int window,
                                         int sinks, float scale, const void *q, int64_t q_stride, void *workspace,
                                         size_t workspace_bytes, void *output, int64_t output_stride);
+size_t camblas_cuda_paged_prefill_workspace_size(const camblas_cuda_context *context, int batch, int tokens, int q_heads,
+                                                 const camblas_cuda_paged_cache *cache, int table_columns, int window,
+                                                 int sinks);
 /* The new tokens of ragged sequences, causal: rows query_starts[b] .. query_starts[b + 1] - 1 of q (int32 [batch + 1] on
  * the device, ascending, at most `tokens`) are sequence b's, the last of them at position lengths[b] - 1; each sees the positions up
  * to its own (or the window and the first tokens, as above). Rows that belong to no sequence are left
- * as they were. */
+ * as they were. The rest, the workspace with its own size among it, as above. */
 int camblas_cuda_paged_prefill_attention(camblas_cuda_context *context, int batch, int tokens, int q_heads,
                                          const camblas_cuda_paged_cache *cache, const int32_t *page_table,
                                          int64_t table_stride, int table_columns, const int32_t *lengths,
                                          const int32_t *query_starts, int window, int sinks, float scale, const void *q,
-                                         int64_t q_stride, void *output, int64_t output_stride);
+                                         int64_t q_stride, void *workspace, size_t workspace_bytes, void *output,
+                                         int64_t output_stride);
 
 /* extension. Planner introspection (the GPU counterpart of the reference CPU planner's
  * camblas_plan_format, src/planner.c:654-669): writes a one-line description of the kernel the

@@ -152,6 +152,14 @@ def test_prefill_windows_and_first_tokens(device, dim, window, sinks):
     check_prefill(device, 1200, [150, 33, 1], [0, 190, 64], q_heads=6, kv_heads=2, dim=dim, page_size=16, window=window, sinks=sinks)
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("new,past,window,sinks", [
+    ([1], [3000], 0, 0), ([1, 17, 0, 40], [3001, 0, 77, 2500], 0, 0), ([9, 3], [2000, 2], 700, 100), ([1] * 5, [1500, 0, 3, 640, 1], 0, 0),
+    ([130], [1300], 1000, 0)])
+def test_prefill_positions_divided_over_workgroups(device, dim, new, past, window, sinks):
+    check_prefill(device, 1250, new, past, q_heads=6, kv_heads=2, dim=dim, page_size=16, window=window, sinks=sinks)
+
+
 @pytest.mark.parametrize("layout", ["together", "heads first"])
 def test_prefill_layouts_of_the_cache(device, layout):
     check_prefill(device, 1300, [40, 100], [10, 0], q_heads=4, kv_heads=2, dim=128, page_size=16, layout=layout)
