@@ -27,7 +27,7 @@ namespace camblas_hip
 {
 namespace
 {
-constexpr int WAVES = 4, THREADS = WAVES * 64, ROWS = WAVES * 32, TILE = 64, JOIN_ROWS = 32, MOST_SHARES = 32;
+constexpr int WAVES = 4, THREADS = WAVES * 64, ROWS = WAVES * 32, TILE = 64, MOST_SHARES = 32;
 constexpr int VECTOR = 0x2, MATRIX = 0x8, DS_READS = 0x100; // kinds of instructions for the scheduler
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -430,36 +430,38 @@ template <int DIM, bool SHARED> __global__ __launch_bounds__(THREADS, DIM == 64 
     }
 }
 
-// Joins the shares of the rows of a block, JOIN_ROWS of them a workgroup, in their order; DIM / 4 threads take a row.
+// Joins the shares of the rows of a block in their order; DIM / 4 threads take a row, and a workgroup as many rows
+// as it has threads for (four rows after each other made 16 us of it where one makes 5).
+template <int DIM> constexpr int join_rows() { return THREADS / (DIM / 4); }
 template <int DIM> __global__ __launch_bounds__(THREADS) void paged_prefill_join_kernel(PrefillParams p)
 {
     constexpr int ROW = DIM / 4;
     Block block;
     if (!find_block(p, blockIdx.x, block))
         return;
+    const int64_t r = int64_t(blockIdx.y) * join_rows<DIM>() + threadIdx.x / ROW;
+    if (r >= block.rows)
+        return;
     const int d = 4 * (threadIdx.x % ROW), q_heads = p.cache.kv_heads * p.group;
-    const int64_t low = int64_t(blockIdx.y) * JOIN_ROWS, high = min(block.rows, low + JOIN_ROWS);
-    for (int64_t r = low + threadIdx.x / ROW; r < high; r += THREADS / ROW) {
-        const int64_t row = block.row0 + r;
-        const int token = block.token0 + int(row / p.group), head = block.kv_head * p.group + int(row % p.group);
-        const size_t first = size_t(token) * q_heads + head, step = size_t(p.tokens) * q_heads;
-        float top = -INFINITY;
+    const int64_t row = block.row0 + r;
+    const int token = block.token0 + int(row / p.group), head = block.kv_head * p.group + int(row % p.group);
+    const size_t first = size_t(token) * q_heads + head, step = size_t(p.tokens) * q_heads;
+    float top = -INFINITY;
 #pragma unroll 4
-        for (int s = 0; s < p.shares; ++s)
-            top = fmaxf(top, p.part_m[first + s * step]);
-        const float reference = top == -INFINITY ? 0.f : top;
-        f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-        float sum = 0.f;
+    for (int s = 0; s < p.shares; ++s)
+        top = fmaxf(top, p.part_m[first + s * step]);
+    const float reference = top == -INFINITY ? 0.f : top;
+    f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+    float sum = 0.f;
 #pragma unroll 4
-        for (int s = 0; s < p.shares; ++s) {
-            const float factor = __builtin_amdgcn_exp2f(p.part_m[first + s * step] - reference);
-            sum = fmaf(factor, p.part_l[first + s * step], sum);
-            o += factor * *reinterpret_cast<const f32x4_t *>(p.part_o + (first + s * step) * DIM + d);
-        }
-        o *= sum == 0.f ? 0.f : 1.f / sum;
-        *reinterpret_cast<u32x2_t *>(p.out + int64_t(token) * p.out_stride + int64_t(head) * DIM + d) =
-            u32x2_t{round_pair(o[0], o[1]), round_pair(o[2], o[3])};
+    for (int s = 0; s < p.shares; ++s) {
+        const float factor = __builtin_amdgcn_exp2f(p.part_m[first + s * step] - reference);
+        sum = fmaf(factor, p.part_l[first + s * step], sum);
+        o += factor * *reinterpret_cast<const f32x4_t *>(p.part_o + (first + s * step) * DIM + d);
     }
+    o *= sum == 0.f ? 0.f : 1.f / sum;
+    *reinterpret_cast<u32x2_t *>(p.out + int64_t(token) * p.out_stride + int64_t(head) * DIM + d) =
+        u32x2_t{round_pair(o[0], o[1]), round_pair(o[2], o[3])};
 }
 
 int64_t prefill_blocks(int batch, int tokens, int group) { return int64_t(tokens) * group / ROWS + batch; }
@@ -531,7 +533,7 @@ hipError_t launch_paged_prefill(hipStream_t stream, int batch, int tokens, int q
     if (status != hipSuccess)
         return status;
     const auto join = dim == 128 ? paged_prefill_join_kernel<128> : paged_prefill_join_kernel<64>;
-    join<<<dim3(numbers, ROWS / JOIN_ROWS), THREADS, 0, stream>>>(p);
+    join<<<dim3(numbers, ROWS / (dim == 128 ? join_rows<128>() : join_rows<64>())), THREADS, 0, stream>>>(p);
     return launch_status();
 }
 } // namespace camblas_hip
