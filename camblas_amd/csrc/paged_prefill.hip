@@ -112,6 +112,24 @@ __device__ __forceinline__ uint64_t below(int count)
     return count <= 0 ? 0 : count >= 64 ? ~uint64_t(0) : (uint64_t(1) << count) - 1;
 }
 
+// eight BF16 values: is one of them NaN or an infinity; those replaced by zero
+__device__ __forceinline__ bool holds_infinite(u32x4_t packed)
+{
+    bool found = false;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        found = found || (packed[e] & 0x7f80u) == 0x7f80u || (packed[e] & 0x7f800000u) == 0x7f800000u;
+    return found;
+}
+__device__ __forceinline__ u32x4_t without_infinite(u32x4_t packed)
+{
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        packed[e] = ((packed[e] & 0x7f80u) == 0x7f80u ? 0 : packed[e] & 0xffffu) |
+                    ((packed[e] & 0x7f800000u) == 0x7f800000u ? 0 : packed[e] & 0xffff0000u);
+    return packed;
+}
+
 // a value that is the same in every lane, in a scalar register
 __device__ __forceinline__ int uniform(int value) { return __builtin_amdgcn_readfirstlane(value); }
 
@@ -159,8 +177,11 @@ template <int DIM, bool SHARED> __global__ __launch_bounds__(THREADS, DIM == 64 
     constexpr int CHUNKS = DIM / 8, FETCH = 64 / CHUNKS, FETCHES = TILE / FETCH / WAVES; // rows of a load, a wavefront's loads
     __shared__ __attribute__((aligned(16))) unsigned char keys0[TILE * DIM * 2], keys1[TILE * DIM * 2];
     __shared__ __attribute__((aligned(16))) unsigned char values0[TILE * DIM * 2], values1[TILE * DIM * 2];
+    __shared__ unsigned infinite[2]; // which rows of a tile hold values that are not finite
     const int thread = threadIdx.x, lane = thread % 64, wave = uniform(thread / 64);
     const int column = lane % 32, half = lane / 32;
+    if (thread < 2)
+        infinite[thread] = 0;
     Block block;
     if (!find_block(p, blockIdx.x, block))
         return;
@@ -186,6 +207,16 @@ template <int DIM, bool SHARED> __global__ __launch_bounds__(THREADS, DIM == 64 
     const TileSpan<TILE> span(p.see, first_query, last_query);
     const int first = SHARED ? int(int64_t(span.tiles) * blockIdx.y / p.shares) : 0;
     const int end = SHARED ? int(int64_t(span.tiles) * (blockIdx.y + 1) / p.shares) : span.tiles;
+
+    // which rows of the tile at hand exist and are seen by some query of the block
+    uint64_t wanted = 0;
+    // bit n: the lane's query sees position base + n
+    const auto seen_rows = [&](int base) {
+        uint64_t seen = wanted & below(query - base + 1);
+        if (p.see.window > 0)
+            seen &= ~below(query - base + 1 - p.see.window) | below(p.see.sinks - base);
+        return seen;
+    };
 
     // ---- fetching tiles: lane r of every wavefront knows the page of tile row r
     const int32_t *pages = p.table.pages + int64_t(sequence) * p.table.stride;
@@ -267,7 +298,6 @@ template <int DIM, bool SHARED> __global__ __launch_bounds__(THREADS, DIM == 64 
     // Turn `tile`: its scores are in `score`, its values in `values`, the keys of the next tile in `next_keys`.
     // Fetched meanwhile: the next tile's values, the keys of the one after. The next tile's scores are multiplied
     // while this one's weights are worked out.
-    uint64_t wanted;
     int page, next_page; // of the rows of the next tile and of the one after
     int64_t at = 0;      // place() of the next tile
     const auto turn = [&](int tile, f32x16_t (&score)[2], f32x16_t (&next_score)[2], unsigned char *keys,
@@ -284,25 +314,30 @@ template <int DIM, bool SHARED> __global__ __launch_bounds__(THREADS, DIM == 64 
         next_page = page_at(tile + 3);
         const bool whole = wanted == ~uint64_t(0) && base + TILE - 1 <= first_query &&
                            (p.see.window <= 0 || base > last_query - p.see.window || base + TILE <= p.see.sinks);
+        uint64_t rows_infinite = 0;
         if (!whole) { // (the same in every wavefront)
-            // bit n: the lane's query sees position base + n
-            uint64_t seen = wanted & below(query - base + 1);
-            if (p.see.window > 0)
-                seen &= ~below(query - base + 1 - p.see.window) | below(p.see.sinks - base);
-            seen >>= 4 * half;
+            const uint64_t own = seen_rows(base) >> (4 * half);
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     // (all bits of a lane's own bit, and a bitwise choice: no masks in scalar registers)
-                    const int keep = __builtin_amdgcn_sbfe(int(seen >> (32 * t)), 8 * (r / 4) + r % 4, 1);
+                    const int keep = __builtin_amdgcn_sbfe(int(own >> (32 * t)), 8 * (r / 4) + r % 4, 1);
                     score[t][r] = __int_as_float((__float_as_int(score[t][r]) & keep) | (int(0xff800000u) & ~keep));
                 }
-            // rows that nobody sees: zeros, which no weight turns into NaN
-            for (int piece = thread; piece < TILE * CHUNKS; piece += THREADS)
-                if (!((wanted >> (piece / CHUNKS)) & 1))
-                    *reinterpret_cast<u32x4_t *>(values + piece * 16) = u32x4_t{0, 0, 0, 0};
+            // A weight of zero times NaN or infinity would reach the output. Rows that nobody sees become zeros. A
+            // row that some see and that holds such values has them taken out of the product and added, as they
+            // are, to the sums of those who see it: no weight changes what becomes of those.
+            for (int piece = thread; piece < TILE * CHUNKS; piece += THREADS) {
+                u32x4_t *at_piece = reinterpret_cast<u32x4_t *>(values + piece * 16);
+                const int r = piece / CHUNKS;
+                if (!((wanted >> r) & 1))
+                    *at_piece = u32x4_t{0, 0, 0, 0};
+                else if (holds_infinite(*at_piece))
+                    atomicOr(&infinite[r / 32], 1u << (r % 32));
+            }
             __syncthreads();
+            rows_infinite = uint64_t(unsigned(uniform(int(infinite[0])))) | uint64_t(unsigned(uniform(int(infinite[1])))) << 32;
         }
         float highest = -INFINITY;
 #pragma unroll
@@ -320,6 +355,37 @@ template <int DIM, bool SHARED> __global__ __launch_bounds__(THREADS, DIM == 64 
 #pragma unroll
             for (int d = 0; d < DIM / 32; ++d)
                 acc[d] *= factor;
+        }
+        if (rows_infinite) {
+            const uint64_t seen = seen_rows(base);
+            for (uint64_t left = rows_infinite; left; left &= left - 1) {
+                const int r = __builtin_ctzll(left);
+                const bool sees_it = (seen >> r) & 1;
+#pragma unroll
+                for (int d = 0; d < DIM / 32; ++d) {
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const int dim = 32 * d + 8 * g + 4 * half;
+                        const u32x2_t packed = *reinterpret_cast<const u32x2_t *>(
+                            values + r * DIM * 2 + ((dim / 8) ^ turn_values<DIM>(r)) * 16 + dim % 8 * 2);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float v = __uint_as_float(e % 2 ? packed[e / 2] & 0xffff0000u : packed[e / 2] << 16);
+                            acc[d][4 * g + e] += sees_it && !(fabsf(v) < INFINITY) ? v : 0.f;
+                        }
+                    }
+                    asm volatile("" ::: "memory"); // (few values at a time in registers)
+                }
+            }
+            __syncthreads();
+            for (int piece = thread; piece < TILE * CHUNKS; piece += THREADS) {
+                u32x4_t *at_piece = reinterpret_cast<u32x4_t *>(values + piece * 16);
+                if (holds_infinite(*at_piece))
+                    *at_piece = without_infinite(*at_piece);
+            }
+            if (thread < 2)
+                infinite[thread] = 0;
+            __syncthreads();
         }
         const float reference = top == -INFINITY ? 0.f : top;
         multiply_keys(next_keys, next_score);

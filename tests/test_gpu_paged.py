@@ -185,6 +185,26 @@ def test_prefill_pages_that_do_not_exist_hold_nothing(device):
     assert reference.within(got, want, allowed) and not got[30:].any()
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("past", [0, 1500])
+def test_prefill_infinite_and_nan_values_reach_only_who_sees_them(device, dim, past):
+    """Rows of the prompt itself that hold NaN and infinities: earlier tokens, and later ones beyond the window, stay
+    finite."""
+    new, window = 200, 70
+    lengths = [past + new]
+    k, v, table = reference.paged_case(1550, lengths, page_size=16, kv_heads=2, dim=dim, device=device)
+    marks = {past + 50: (3, math.nan), past + 51: (4, math.inf), past + 127: (dim - 1, -math.inf), past + 128: (9, math.inf)}
+    for position, (d, value) in marks.items():
+        v[int(table[0, position // 16]), position % 16, 1, d] = value
+    k[int(table[0, (past + 160) // 16]), (past + 160) % 16, 0, 2] = math.nan
+    q = queries(1551, new, 6, dim, device)
+    got = _kernels.paged_prefill_attention(q, k, v, table, torch.tensor(lengths, dtype=torch.int32, device=device), starts_of([new], device),
+                                           window=window, sinks=0)
+    want, allowed = reference.attention_rows(q, k, v, table, lengths, [new], window=window, sinks=0)
+    assert reference.within(got, want, allowed)
+    assert torch.isnan(want).any() and torch.isinf(want).any()
+
+
 def test_prefill_one_token_each_equals_decode_within_rounding(device):
     lengths = [1, 70, 1030, 257]
     k, v, table = reference.paged_case(1600, lengths, page_size=16, kv_heads=2, dim=128, device=device)
