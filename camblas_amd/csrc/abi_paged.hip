@@ -52,7 +52,7 @@ bool valid_attention(int batch, int tokens, int q_heads, const camblas_cuda_page
                      int table_columns, int window, int sinks, float scale, int64_t q_stride, int64_t output_stride)
 {
     return valid_heads(q_heads, cache) && within({{batch, 0, 65535, 1}, {tokens, 0, INT32_MAX, 1}, {window, 0, INT32_MAX, 1},
-                                                  {sinks, 0, INT32_MAX, 1},
+                                                  {sinks, 0, INT32_MAX, 1}, {int64_t(tokens) * q_heads, 0, int64_t(1) << 30, 1},
                                                   {int64_t(table_columns) * cache->page_size, 0, int64_t(1) << 30, 1}}) &&
            table_columns >= 0 && table_stride >= (batch > 1 ? table_columns : 0) && std::isfinite(scale) && scale > 0.f &&
            scale < 1e30f && q_stride % 8 == 0 && output_stride % 8 == 0 &&

@@ -141,7 +141,7 @@ __device__ __forceinline__ int first_token(const PrefillParams &p, int sequence)
 // A block of ROWS rows of one key-value head: row r of it is query head r % group of token r / group.
 struct Block {
     int sequence, kv_head, token0, tokens; // the sequence's first token and how many it has
-    int64_t row0, rows;                    // the block's first row, how many rows the sequence has from there on
+    int row0, rows;                        // the block's first row, how many rows the sequence has from there on
 };
 
 // Blocks of sequence b are numbered from floor(first token * group / ROWS) + b: a number that needs no
@@ -157,8 +157,9 @@ __device__ __forceinline__ bool find_block(const PrefillParams &p, int number, B
         found = 0;
     __syncthreads();
     for (int b = threadIdx.x; b < p.batch; b += THREADS) {
-        const int64_t here = int64_t(first_token(p, b)) * p.group / ROWS + b;
-        const int64_t next = int64_t(first_token(p, b + 1)) * p.group / ROWS + b + 1;
+        // (tokens * query heads is at most 2^30)
+        const int here = first_token(p, b) * p.group / ROWS + b;
+        const int next = first_token(p, b + 1) * p.group / ROWS + b + 1;
         if (here <= wanted && wanted < next)
             found = b;
     }
@@ -166,8 +167,8 @@ __device__ __forceinline__ bool find_block(const PrefillParams &p, int number, B
     block.sequence = uniform(found);
     block.token0 = uniform(first_token(p, block.sequence));
     block.tokens = uniform(first_token(p, block.sequence + 1)) - block.token0;
-    block.row0 = (wanted - (int64_t(block.token0) * p.group / ROWS + block.sequence)) * ROWS;
-    block.rows = int64_t(block.tokens) * p.group - block.row0;
+    block.row0 = (wanted - (block.token0 * p.group / ROWS + block.sequence)) * ROWS;
+    block.rows = block.tokens * p.group - block.row0;
     return block.row0 >= 0 && block.rows > 0;
 }
 
@@ -186,24 +187,23 @@ template <int DIM, bool SHARED> __global__ __launch_bounds__(THREADS, DIM == 64 
     if (!find_block(p, blockIdx.x, block))
         return;
     const int sequence = block.sequence, kv_head = block.kv_head, token0 = block.token0, tokens = block.tokens;
-    const int64_t row0 = block.row0, rows = block.rows;
+    const int row0 = block.row0, rows = block.rows;
 
     // ---- this lane's row: token and query head, position
     const int past = uniform(live_positions(p.table, p.cache, sequence)) - tokens;
     int query;
     bf16x8_t q[DIM / 16];
     {
-        const int64_t row = row0 + wave * 32 + column;
-        const int64_t kept = row < rows + row0 ? row : rows + row0 - 1;
-        const int token = int(kept / p.group), head = kv_head * p.group + int(kept % p.group);
+        const unsigned row = unsigned(min(row0 + wave * 32 + column, row0 + rows - 1)), group = p.group;
+        const int token = int(row / group), head = kv_head * p.group + int(row % group);
         query = past + token;
         const unsigned short *from = p.q + int64_t(token0 + token) * p.q_stride + int64_t(head) * DIM + 8 * half;
 #pragma unroll
         for (int s = 0; s < DIM / 16; ++s)
             q[s] = *reinterpret_cast<const bf16x8_t *>(from + 16 * s);
     }
-    const int first_query = uniform(past + int(row0 / p.group));
-    const int last_query = uniform(past + int((row0 + min(rows, int64_t(ROWS)) - 1) / p.group));
+    const int first_query = uniform(past + int(unsigned(row0) / unsigned(p.group)));
+    const int last_query = uniform(past + int(unsigned(row0 + min(rows, ROWS) - 1) / unsigned(p.group)));
     const TileSpan<TILE> span(p.see, first_query, last_query);
     const int first = SHARED ? int(int64_t(span.tiles) * blockIdx.y / p.shares) : 0;
     const int end = SHARED ? int(int64_t(span.tiles) * (blockIdx.y + 1) / p.shares) : span.tiles;
@@ -464,11 +464,12 @@ template <int DIM, bool SHARED> __global__ __launch_bounds__(THREADS, DIM == 64 
         }
     }
 
-    const int64_t row = row0 + wave * 32 + column;
+    const int row = row0 + wave * 32 + column;
     const float sum = total + __shfl_xor(total, 32);
     if (row >= row0 + rows)
         return;
-    const int token = token0 + int(row / p.group), head = kv_head * p.group + int(row % p.group);
+    const int token = token0 + int(unsigned(row) / unsigned(p.group));
+    const int head = kv_head * p.group + int(unsigned(row) % unsigned(p.group));
     if constexpr (SHARED) {
         const size_t at_row = (size_t(blockIdx.y) * p.tokens + token) * (p.cache.kv_heads * p.group) + head;
         if (half == 0) {
@@ -505,12 +506,12 @@ template <int DIM> __global__ __launch_bounds__(THREADS) void paged_prefill_join
     Block block;
     if (!find_block(p, blockIdx.x, block))
         return;
-    const int64_t r = int64_t(blockIdx.y) * join_rows<DIM>() + threadIdx.x / ROW;
+    const int r = int(blockIdx.y * join_rows<DIM>() + threadIdx.x / ROW);
     if (r >= block.rows)
         return;
     const int d = 4 * (threadIdx.x % ROW), q_heads = p.cache.kv_heads * p.group;
-    const int64_t row = block.row0 + r;
-    const int token = block.token0 + int(row / p.group), head = block.kv_head * p.group + int(row % p.group);
+    const unsigned row = unsigned(block.row0 + r), group = p.group;
+    const int token = block.token0 + int(row / group), head = block.kv_head * p.group + int(row % group);
     const size_t first = size_t(token) * q_heads + head, step = size_t(p.tokens) * q_heads;
     float top = -INFINITY;
 #pragma unroll 4

@@ -398,7 +398,8 @@ int camblas_cuda_fp8_moe_decode(camblas_cuda_context *context, int experts, int 
  *
  * A sequence's row of a page table (int32 [batch][table_columns], table_stride apart) maps its position p to
  * page table[p / page_size], slot p % page_size. Entries outside [0, pages) hold nothing: such positions are
- * neither read nor attended to. table_columns * page_size is at most 2^30; lengths are clipped to it. */
+ * neither read nor attended to. table_columns * page_size is at most 2^30; lengths are clipped to it. Query rows times q_heads are at
+ * most 2^30. */
 typedef struct camblas_cuda_paged_cache {
     void *k, *v;
     int64_t page_stride, slot_stride, head_stride;
