@@ -47,6 +47,11 @@ bool valid_heads(int q_heads, const camblas_cuda_paged_cache *cache)
     return q_heads >= 1 && q_heads <= 65536 && q_heads % cache->kv_heads == 0;
 }
 
+Visibility visible(const camblas_cuda_paged_cache *cache, int table_columns, int window, int sinks)
+{
+    return clipped(window, sinks, int64_t(table_columns) * cache->page_size);
+}
+
 // What both attentions ask of their arguments, `batch` sequences and `tokens` query rows.
 bool valid_attention(int batch, int tokens, int q_heads, const camblas_cuda_paged_cache *cache, int64_t table_stride,
                      int table_columns, int window, int sinks, float scale, int64_t q_stride, int64_t output_stride)
@@ -102,7 +107,7 @@ extern "C" size_t camblas_cuda_paged_decode_workspace_size(const camblas_cuda_co
                          int64_t(q_heads) * cache->dim, int64_t(q_heads) * cache->dim))
         return 0;
     return paged_decode_workspace(batch, q_heads, cache->kv_heads, cache->dim, int64_t(table_columns) * cache->page_size,
-                                  window, sinks, context->compute_units);
+                                  visible(cache, table_columns, window, sinks), context->compute_units);
 }
 
 extern "C" int camblas_cuda_paged_decode_attention(camblas_cuda_context *context, int batch, int q_heads,
@@ -125,14 +130,14 @@ extern "C" int camblas_cuda_paged_decode_attention(camblas_cuda_context *context
             !apart(output, {q, cache->k, cache->v, page_table, lengths}))
             return entry.refuse("invalid paged attention buffers");
         const size_t bytes = paged_decode_workspace(batch, q_heads, cache->kv_heads, cache->dim,
-                                                    int64_t(table_columns) * cache->page_size, window, sinks,
-                                                    context->compute_units);
+                                                    int64_t(table_columns) * cache->page_size,
+                                  visible(cache, table_columns, window, sinks), context->compute_units);
         if (bytes && (!usable({{workspace, 16}}) || workspace_bytes < bytes))
             return entry.refuse("paged attention workspace is missing, misaligned or too small");
         context->counts[6]++;
         return entry.finish(launch_paged_decode(entry.stream(), batch, q_heads, cache->dim, device_cache(cache),
                                                 PageTable{page_table, lengths, table_stride, table_columns},
-                                                Visibility{window, sinks}, scale, q, q_stride, output, output_stride,
+                                                visible(cache, table_columns, window, sinks), scale, q, q_stride, output, output_stride,
                                                 workspace, context->compute_units),
                             "paged decode attention");
     });
@@ -147,7 +152,8 @@ extern "C" size_t camblas_cuda_paged_prefill_workspace_size(const camblas_cuda_c
                          int64_t(q_heads) * cache->dim, int64_t(q_heads) * cache->dim))
         return 0;
     return paged_prefill_workspace(batch, tokens, q_heads, cache->kv_heads, cache->dim,
-                                   int64_t(table_columns) * cache->page_size, window, sinks, context->compute_units);
+                                   int64_t(table_columns) * cache->page_size,
+                                  visible(cache, table_columns, window, sinks), context->compute_units);
 }
 
 extern "C" int camblas_cuda_paged_prefill_attention(camblas_cuda_context *context, int batch, int tokens, int q_heads,
@@ -170,14 +176,14 @@ extern "C" int camblas_cuda_paged_prefill_attention(camblas_cuda_context *contex
             !apart(output, {q, cache->k, cache->v, page_table, lengths, query_starts}))
             return entry.refuse("invalid paged attention buffers");
         const size_t bytes = paged_prefill_workspace(batch, tokens, q_heads, cache->kv_heads, cache->dim,
-                                                     int64_t(table_columns) * cache->page_size, window, sinks,
-                                                     context->compute_units);
+                                                     int64_t(table_columns) * cache->page_size,
+                                  visible(cache, table_columns, window, sinks), context->compute_units);
         if (bytes && (!usable({{workspace, 16}}) || workspace_bytes < bytes))
             return entry.refuse("paged attention workspace is missing, misaligned or too small");
         context->counts[6]++;
         return entry.finish(launch_paged_prefill(entry.stream(), batch, tokens, q_heads, cache->dim, device_cache(cache),
                                                  PageTable{page_table, lengths, table_stride, table_columns},
-                                                 Visibility{window, sinks}, query_starts, scale, q, q_stride, output,
+                                                 visible(cache, table_columns, window, sinks), query_starts, scale, q, q_stride, output,
                                                  output_stride, workspace, context->compute_units),
                             "paged prefill attention");
     });

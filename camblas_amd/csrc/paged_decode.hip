@@ -383,8 +383,8 @@ template <int DIM, bool LARGE> __global__ __launch_bounds__(SHARE_WAVES * 64, 2)
     const int64_t workers = min(all, int64_t(gridDim.x)); // each has a step, at least
     if (int64_t(blockIdx.x) >= workers)
         return; // (uniform)
-    int64_t step = all * blockIdx.x / workers;
-    const int64_t stop = all * (blockIdx.x + 1) / workers;
+    int64_t step = share_begin(all, workers, blockIdx.x);
+    const int64_t stop = share_begin(all, workers, int64_t(blockIdx.x) + 1);
     if (step >= before && step < before + mine) {
         for (int b = from; b < to; ++b) {
             int query;
@@ -411,9 +411,8 @@ template <int DIM, bool LARGE> __global__ __launch_bounds__(SHARE_WAVES * 64, 2)
             const int last = int(min(int64_t(steps), stop - begins));
             const int slot = first > 0 ? 2 * int(blockIdx.x) : last < steps ? 2 * int(blockIdx.x) + 1 : -1;
             if (first == 0 && thread == 0) {
-                // the workgroup that holds step s is the last whose run starts at or before it
-                const int64_t ends = ((begins + steps) * workers - 1) / all;
-                p.joins[size_t(sequence) * items + index] = int2{int(blockIdx.x), int(ends)};
+                p.joins[size_t(sequence) * items + index] =
+                    int2{int(blockIdx.x), int(share_of(all, workers, begins + steps - 1))};
             }
             work_item<DIM, LARGE, WAVES>(p, queries, scale, item_of(p, sequence, index), span, query, first, last,
                                   first_page<WAVES>(p, span, sequence, first), slot);
@@ -512,11 +511,11 @@ static int64_t decode_positions(int64_t capacity, const Visibility &see)
     return see.window > 0 && int64_t(see.window) + see.sinks < capacity ? int64_t(see.window) + see.sinks : capacity;
 }
 
-size_t paged_decode_workspace(int batch, int q_heads, int kv_heads, int dim, int64_t capacity, int window, int sinks,
+size_t paged_decode_workspace(int batch, int q_heads, int kv_heads, int dim, int64_t capacity, const Visibility &see,
                               int compute_units)
 {
     const int64_t items = int64_t(batch) * kv_heads * ((q_heads / kv_heads + HEADS - 1) / HEADS);
-    const size_t shares = size_t(decode_shares(items, decode_positions(capacity, Visibility{window, sinks}), compute_units));
+    const size_t shares = size_t(decode_shares(items, decode_positions(capacity, see), compute_units));
     return shares ? 2 * shares * HEADS * (size_t(dim) + 2) * sizeof(float) + size_t(items) * sizeof(int2) : 0;
 }
 

@@ -144,9 +144,7 @@ struct Block {
     int row0, rows;                        // the block's first row, how many rows the sequence has from there on
 };
 
-// Blocks of sequence b are numbered from floor(first token * group / ROWS) + b: a number that needs no
-// sum over the sequences before, leaves room for a last block that is not full, and at most one unused
-// number per sequence. False for an unused number.
+// The block of a number (first_block); false for one that is not used.
 __device__ __forceinline__ bool find_block(const PrefillParams &p, int number, Block &block)
 {
     __shared__ int found;
@@ -157,9 +155,8 @@ __device__ __forceinline__ bool find_block(const PrefillParams &p, int number, B
         found = 0;
     __syncthreads();
     for (int b = threadIdx.x; b < p.batch; b += THREADS) {
-        // (tokens * query heads is at most 2^30)
-        const int here = first_token(p, b) * p.group / ROWS + b;
-        const int next = first_token(p, b + 1) * p.group / ROWS + b + 1;
+        const int here = first_block(first_token(p, b), p.group, ROWS, b);
+        const int next = first_block(first_token(p, b + 1), p.group, ROWS, b + 1);
         if (here <= wanted && wanted < next)
             found = b;
     }
@@ -167,7 +164,7 @@ __device__ __forceinline__ bool find_block(const PrefillParams &p, int number, B
     block.sequence = uniform(found);
     block.token0 = uniform(first_token(p, block.sequence));
     block.tokens = uniform(first_token(p, block.sequence + 1)) - block.token0;
-    block.row0 = (wanted - (block.token0 * p.group / ROWS + block.sequence)) * ROWS;
+    block.row0 = (wanted - first_block(block.token0, p.group, ROWS, block.sequence)) * ROWS;
     block.rows = block.tokens * p.group - block.row0;
     return block.row0 >= 0 && block.rows > 0;
 }
@@ -551,12 +548,12 @@ int64_t prefill_positions(int64_t capacity, const Visibility &see, int tokens, i
 }
 } // namespace
 
-size_t paged_prefill_workspace(int batch, int tokens, int q_heads, int kv_heads, int dim, int64_t capacity, int window, int sinks,
-                               int compute_units)
+size_t paged_prefill_workspace(int batch, int tokens, int q_heads, int kv_heads, int dim, int64_t capacity,
+                               const Visibility &see, int compute_units)
 {
     const int group = q_heads / kv_heads;
     const int shares = prefill_shares(prefill_blocks(batch, tokens, group) * kv_heads, dim,
-                                      prefill_positions(capacity, Visibility{window, sinks}, tokens, group), compute_units);
+                                      prefill_positions(capacity, see, tokens, group), compute_units);
     return shares > 1 ? size_t(shares) * tokens * q_heads * (size_t(dim) + 2) * sizeof(float) : 0;
 }
 
