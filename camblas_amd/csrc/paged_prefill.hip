@@ -141,32 +141,38 @@ __device__ __forceinline__ int first_token(const PrefillParams &p, int sequence)
 // A block of ROWS rows of one key-value head: row r of it is query head r % group of token r / group.
 struct Block {
     int sequence, kv_head, token0, tokens; // the sequence's first token and how many it has
+    int length;                            // positions of the sequence
     int row0, rows;                        // the block's first row, how many rows the sequence has from there on
 };
 
-// The block of a number (first_block); false for one that is not used.
+// The block of a number (first_block); false for one that is not used. The lengths travel with the starts: a
+// small call is a chain of trips to memory.
 __device__ __forceinline__ bool find_block(const PrefillParams &p, int number, Block &block)
 {
-    __shared__ int found;
+    __shared__ int found[4];
     // the last blocks of a causal sequence see most: they start first
     block.kv_head = number % p.cache.kv_heads;
     const int wanted = p.row_blocks - 1 - number / p.cache.kv_heads;
     if (threadIdx.x == 0)
-        found = 0;
+        found[0] = -1;
     __syncthreads();
     for (int b = threadIdx.x; b < p.batch; b += THREADS) {
-        const int here = first_block(first_token(p, b), p.group, ROWS, b);
-        const int next = first_block(first_token(p, b + 1), p.group, ROWS, b + 1);
-        if (here <= wanted && wanted < next)
-            found = b;
+        const int begin = first_token(p, b), end = first_token(p, b + 1), length = live_positions(p.table, p.cache, b);
+        if (first_block(begin, p.group, ROWS, b) <= wanted && wanted < first_block(end, p.group, ROWS, b + 1)) {
+            found[0] = b;
+            found[1] = begin;
+            found[2] = end - begin;
+            found[3] = length;
+        }
     }
     __syncthreads();
-    block.sequence = uniform(found);
-    block.token0 = uniform(first_token(p, block.sequence));
-    block.tokens = uniform(first_token(p, block.sequence + 1)) - block.token0;
+    block.sequence = uniform(found[0]);
+    block.token0 = uniform(found[1]);
+    block.tokens = uniform(found[2]);
+    block.length = uniform(found[3]);
     block.row0 = (wanted - first_block(block.token0, p.group, ROWS, block.sequence)) * ROWS;
     block.rows = block.tokens * p.group - block.row0;
-    return block.row0 >= 0 && block.rows > 0;
+    return block.sequence >= 0 && block.row0 >= 0 && block.rows > 0;
 }
 
 // SHARED: blockIdx.y of `shares` workgroups takes its part of the tiles and leaves what it has for the join.
@@ -187,7 +193,7 @@ template <int DIM, bool SHARED> __global__ __launch_bounds__(THREADS, DIM == 64 
     const int row0 = block.row0, rows = block.rows;
 
     // ---- this lane's row: token and query head, position
-    const int past = uniform(live_positions(p.table, p.cache, sequence)) - tokens;
+    const int past = block.length - tokens;
     int query;
     bf16x8_t q[DIM / 16];
     {
