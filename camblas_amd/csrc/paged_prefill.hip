@@ -112,6 +112,12 @@ __device__ __forceinline__ uint64_t below(int count)
     return count <= 0 ? 0 : count >= 64 ? ~uint64_t(0) : (uint64_t(1) << count) - 1;
 }
 
+// The upper 32 lanes of `first` against the lower 32 of `second`.
+__device__ __forceinline__ u32x2_t swap_halves(unsigned first, unsigned second)
+{
+    return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_permlane32_swap(first, second, false, false));
+}
+
 // eight BF16 values: is one of them NaN or an infinity; those replaced by zero
 __device__ __forceinline__ bool holds_infinite(u32x4_t packed)
 {
@@ -469,11 +475,12 @@ template <int DIM, bool SHARED> __global__ __launch_bounds__(THREADS, DIM == 64 
 
     const int row = row0 + wave * 32 + column;
     const float sum = total + __shfl_xor(total, 32);
-    if (row >= row0 + rows)
-        return;
+    const bool kept = row < row0 + rows; // (the others' lanes still take part in the exchange)
     const int token = token0 + int(unsigned(row) / unsigned(p.group));
     const int head = kv_head * p.group + int(unsigned(row) % unsigned(p.group));
     if constexpr (SHARED) {
+        if (!kept)
+            return;
         const size_t at_row = (size_t(blockIdx.y) * p.tokens + token) * (p.cache.kv_heads * p.group) + head;
         if (half == 0) {
             p.part_m[at_row] = top;
@@ -489,14 +496,25 @@ template <int DIM, bool SHARED> __global__ __launch_bounds__(THREADS, DIM == 64 
     } else {
         // (no position seen: zero; a sum that is NaN stays NaN)
         const float inverse = sum == 0.f ? 0.f : 1.f / sum;
-        unsigned short *to = p.out + int64_t(token) * p.out_stride + int64_t(head) * DIM + 4 * half;
+        // The two lanes of a row hold four dims each of every eight: the upper gives its half of the even eights for
+        // the lower's half of the odd ones, and each writes eight dims in one piece.
+        unsigned short *to = p.out + int64_t(token) * p.out_stride + int64_t(head) * DIM + 8 * half;
 #pragma unroll
         for (int d = 0; d < DIM / 32; ++d)
 #pragma unroll
-            for (int g = 0; g < 4; ++g)
-                *reinterpret_cast<u32x2_t *>(to + 32 * d + 8 * g) =
-                    u32x2_t{round_pair(acc[d][4 * g] * inverse, acc[d][4 * g + 1] * inverse),
-                            round_pair(acc[d][4 * g + 2] * inverse, acc[d][4 * g + 3] * inverse)};
+            for (int g = 0; g < 4; g += 2) {
+                u32x4_t whole;
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const unsigned even = round_pair(acc[d][4 * g + 2 * e] * inverse, acc[d][4 * g + 2 * e + 1] * inverse);
+                    const unsigned odd = round_pair(acc[d][4 * g + 4 + 2 * e] * inverse, acc[d][4 * g + 5 + 2 * e] * inverse);
+                    const u32x2_t swapped = swap_halves(even, odd);
+                    whole[e] = swapped[0];
+                    whole[2 + e] = swapped[1];
+                }
+                if (kept)
+                    *reinterpret_cast<u32x4_t *>(to + 32 * d + 8 * g) = whole;
+            }
     }
 }
 
