@@ -39,7 +39,7 @@ struct AppendParams {
     unsigned short *q_out;
     int64_t token_stride, out_stride;
     PagedCache cache;
-    double turns[64]; // theta^(-2 i / rotary) / (2 pi)
+    double powers[6]; // theta^(-2 i / rotary) for i = 1, 2, 4, .. 32
 };
 
 __device__ __forceinline__ void load_weights(const void *weight, int bf16, int at, float (&w)[8])
@@ -92,7 +92,12 @@ template <int DIM> __global__ __launch_bounds__(APPEND_WAVES * 64) void qk_norm_
     __shared__ __attribute__((aligned(16))) float sines[APPEND_WAVES][64], cosines[APPEND_WAVES][64];
     const int wave = threadIdx.x / 64;
     {
-        const double turn = double(p.positions[token]) * p.turns[lane];
+        // theta^(-2 lane / rotary) as a product over the bits of the lane (64 values worked out on the host were 2 of
+        // the 6 us of a small call); twelve roundings of 2^-53 are lost in that of the turn
+        double turn = double(p.positions[token]) * (1 / 6.283185307179586476925);
+#pragma unroll
+        for (int bit = 0; bit < 6; ++bit)
+            turn *= lane >> bit & 1 ? p.powers[bit] : 1.0;
         float s, c;
         sincospif(2.f * float(turn - rint(turn)), &s, &c);
         sines[wave][lane] = s;
@@ -203,13 +208,10 @@ hipError_t launch_qk_norm_rope_append(hipStream_t stream, int tokens, int q_head
     p.token_stride = token_stride;
     p.out_stride = out_stride;
     p.cache = cache;
-    // (by products: 64 powers were 1.3 us of a 6 us call; a product's rounding, 2^-53 a step, is lost in that of
-    // position times turn)
-    double turn = 1 / 6.283185307179586476925;
-    const double ratio = rotary ? std::pow(double(theta), -2.0 / rotary) : 1;
-    for (int i = 0; i < p.half; ++i) {
-        p.turns[i] = turn;
-        turn *= ratio;
+    double power = rotary ? std::pow(double(theta), -2.0 / rotary) : 1;
+    for (double &of : p.powers) {
+        of = power;
+        power *= power;
     }
     const int heads = q_heads + 2 * cache.kv_heads, at_once = 1024 / dim;
     const int groups = (heads + at_once - 1) / at_once;
