@@ -790,7 +790,7 @@ def _tensor_binding():
 
 
 # The paged cache's operators go through the tensor binding: a decode step's kernels take a few microseconds,
-# less than checking and passing a dozen arguments through ctypes (16 against 6 us a call).
+# less than checking and passing a dozen arguments through ctypes (16 against 5 us a call).
 
 
 def qk_norm_rope_append(qkv, positions, slots, k_cache, v_cache, *, q_heads, kv_heads, q_weight=None, k_weight=None,

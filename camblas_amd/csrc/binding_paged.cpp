@@ -10,9 +10,11 @@ namespace
 {
 camblas_cuda_paged_cache pages_of(const Tensor &k, const Tensor &v, const at::Device &device)
 {
-    require(k.scalar_type() == at::kBFloat16 && v.scalar_type() == at::kBFloat16 && k.dim() == 4 &&
-                k.sizes().equals(v.sizes()) && k.strides().equals(v.strides()) && k.device() == device &&
-                v.device() == device,
+    bool alike = k.scalar_type() == at::kBFloat16 && v.scalar_type() == at::kBFloat16 && k.dim() == 4 &&
+                 k.sizes().equals(v.sizes()) && k.device() == device && v.device() == device;
+    for (int axis = 0; alike && axis < 4; ++axis)
+        alike = k.size(axis) < 2 || k.stride(axis) == v.stride(axis);
+    require(alike,
             "a paged cache is two BF16 tensors [pages, page_size, kv_heads, dim] of one layout on the operands' device");
     require(!recording(k) && !recording(v), "the paged cache's operators support inference only");
     require(k.size(0) >= 1 && k.size(0) <= INT_MAX && k.size(1) <= INT_MAX && k.size(2) <= INT_MAX &&
@@ -21,9 +23,10 @@ camblas_cuda_paged_cache pages_of(const Tensor &k, const Tensor &v, const at::De
     camblas_cuda_paged_cache cache = {};
     cache.k = k.data_ptr();
     cache.v = v.data_ptr();
-    cache.page_stride = k.stride(0);
-    cache.slot_stride = k.stride(1);
-    cache.head_stride = k.stride(2);
+    // (the stride of an axis of one element says nothing)
+    cache.page_stride = k.size(0) > 1 ? k.stride(0) : 0;
+    cache.slot_stride = k.size(1) > 1 ? k.stride(1) : 0;
+    cache.head_stride = k.size(2) > 1 ? k.stride(2) : 0;
     cache.pages = int(k.size(0));
     cache.page_size = int(k.size(1));
     cache.kv_heads = int(k.size(2));
@@ -42,7 +45,7 @@ int64_t row_stride(const char *role, const Tensor &rows, int64_t tokens, int64_t
                                     std::to_string(heads) + ", " + std::to_string(dim) +
                                     "] with dense heads on the operands' GPU");
     require(!recording(rows), "the paged cache's operators support inference only");
-    return rows.stride(0);
+    return tokens > 1 ? rows.stride(0) : heads * dim;
 }
 
 void check_integers(const char *role, const Tensor &values, at::ScalarType type, int64_t count, const at::Device &device)
@@ -106,7 +109,7 @@ struct Attention {
     camblas_cuda_paged_cache cache;
     at::Device device;
     int batch, columns, tokens, q_heads, window, sinks;
-    int64_t q_stride, output_stride;
+    int64_t q_stride, output_stride, table_stride;
     float scale;
     Tensor output;
 
@@ -123,6 +126,7 @@ struct Attention {
         q_stride = row_stride("q", q, q.size(0), q.size(1), cache.dim, device);
         batch = int(page_table.size(0));
         columns = int(page_table.size(1));
+        table_stride = batch > 1 ? page_table.stride(0) : columns;
         tokens = int(q.size(0));
         q_heads = int(q.size(1));
         window = as_int("window", window_in);
@@ -145,7 +149,7 @@ Tensor decode(const Tensor &q, const Tensor &k_cache, const Tensor &v_cache, con
     if (bytes)
         workspace = at::empty({int64_t(bytes)}, q.options().dtype(at::kByte));
     succeed(camblas_cuda_paged_decode_attention(
-                context, a.batch, a.q_heads, &a.cache, page_table.const_data_ptr<int32_t>(), page_table.stride(0), a.columns,
+                context, a.batch, a.q_heads, &a.cache, page_table.const_data_ptr<int32_t>(), a.table_stride, a.columns,
                 lengths.const_data_ptr<int32_t>(), a.window, a.sinks, a.scale, q.const_data_ptr(), a.q_stride,
                 bytes ? workspace.mutable_data_ptr() : nullptr, bytes, a.output.mutable_data_ptr(), a.output_stride),
             context);
@@ -166,7 +170,7 @@ Tensor prefill(const Tensor &q, const Tensor &k_cache, const Tensor &v_cache, co
     if (bytes)
         workspace = at::empty({int64_t(bytes)}, q.options().dtype(at::kByte));
     succeed(camblas_cuda_paged_prefill_attention(
-                context, a.batch, a.tokens, a.q_heads, &a.cache, page_table.const_data_ptr<int32_t>(), page_table.stride(0),
+                context, a.batch, a.tokens, a.q_heads, &a.cache, page_table.const_data_ptr<int32_t>(), a.table_stride,
                 a.columns, lengths.const_data_ptr<int32_t>(), query_starts.const_data_ptr<int32_t>(), a.window, a.sinks,
                 a.scale, q.const_data_ptr(), a.q_stride, bytes ? workspace.mutable_data_ptr() : nullptr, bytes,
                 a.output.mutable_data_ptr(), a.output_stride),

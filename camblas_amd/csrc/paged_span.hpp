@@ -90,6 +90,32 @@ template <int TILE> struct TileSpan {
     }
 };
 
+// Rows of `width` elements, `stride` apart.
+struct Rows {
+    const unsigned short *first;
+    int64_t count, width, stride;
+};
+
+// Whether no element of one lies in the other. Rows of one stride may lie between each other (heads of one
+// activation); of different strides they may not even interleave.
+inline bool rows_apart(const Rows &a, const Rows &b)
+{
+    if (a.count <= 0 || b.count <= 0)
+        return true;
+    const uintptr_t a_begin = reinterpret_cast<uintptr_t>(a.first), b_begin = reinterpret_cast<uintptr_t>(b.first);
+    const uintptr_t a_end = a_begin + uintptr_t((a.count - 1) * a.stride + a.width) * sizeof(unsigned short);
+    const uintptr_t b_end = b_begin + uintptr_t((b.count - 1) * b.stride + b.width) * sizeof(unsigned short);
+    if (a_end <= b_begin || b_end <= a_begin)
+        return true;
+    const int64_t stride = a.count > 1 ? a.stride : b.stride;
+    if (stride <= 0 || (a.count > 1 && b.count > 1 && a.stride != b.stride))
+        return false;
+    const int64_t bytes = stride * int64_t(sizeof(unsigned short));
+    int64_t along = (int64_t(b_begin) - int64_t(a_begin)) % bytes; // of b's rows inside a's
+    along += along < 0 ? bytes : 0;
+    return along >= a.width * int64_t(sizeof(unsigned short)) && along + b.width * int64_t(sizeof(unsigned short)) <= bytes;
+}
+
 // `all` steps dealt to `workers` (at most as many) in runs that differ by one step at most: the first step of
 // worker g's run, and the worker that holds a step.
 PAGED_INLINE int64_t share_begin(int64_t all, int64_t workers, int64_t g) { return all * g / workers; }

@@ -398,8 +398,9 @@ int camblas_cuda_fp8_moe_decode(camblas_cuda_context *context, int experts, int 
  *
  * A sequence's row of a page table (int32 [batch][table_columns], table_stride apart) maps its position p to
  * page table[p / page_size], slot p % page_size. Entries outside [0, pages) hold nothing: such positions are
- * neither read nor attended to. table_columns * page_size is at most 2^30; lengths are clipped to it. Query rows times q_heads are at
- * most 2^30. */
+ * neither read nor attended to. table_columns * page_size is at most 2^30; lengths are clipped to it. Query
+ * rows times q_heads are at most 2^30, the tokens of one append 2^25. Rows that are written share no memory
+ * with those that are read, except as stated. */
 typedef struct camblas_cuda_paged_cache {
     void *k, *v;
     int64_t page_stride, slot_stride, head_stride;
@@ -409,8 +410,8 @@ typedef struct camblas_cuda_paged_cache {
 /* Between a decoder layer's QKV product and its attention, in one launch. qkv holds un-rotated rows
  * [q_heads | kv_heads (k) | kv_heads (v)] of dim values, token_stride elements apart. Query and key heads are
  * normalised, x * rsqrt(mean(x^2) + epsilon) * weight over each head (q_weight, k_weight [dim], both or
- * neither, 16-byte aligned; weight_dtype 0 FP32, 2 BF16), then rotated by halves over their first rotary_dim (a multiple of 16,
- * 0: none) dims by positions[token] * theta^(-2i / rotary_dim); all in FP32 with the angle in FP64, and
+ * neither, 16-byte aligned; weight_dtype 0 FP32, 2 BF16), then rotated by halves over their first rotary_dim
+ * (a multiple of 16, 0: none) dims by positions[token] * theta^(-2i / rotary_dim); all in FP32 with the angle in FP64, and
  * rounded to BF16 once. The queries go to `queries` (rows of q_heads * dim, queries_stride apart; it may be
  * qkv itself with its stride), keys and values to the slot slots[token] = page * page_size + place of every
  * token. A slot outside the cache writes nothing (padding rows: -1); of two tokens with one slot either may
@@ -424,8 +425,8 @@ int camblas_cuda_qk_norm_rope_append(camblas_cuda_context *context, int tokens, 
  * lengths[b] - 1, over its sequence's positions: all of them (window 0), or the last `window` and the first
  * `sinks`. output = softmax(scale q k^T) v per head, scale positive; FP32 sums, weights rounded to BF16 for the
  * second product, one rounding at the end; zeros where a token sees nothing. The cache's rows that a token does
- * not see do not reach its output, whatever they hold. workspace: ..._workspace_size() bytes (0: none), 16-byte aligned, written
- * before it is read; calls that may run at the same time need one each. No atomics: results repeat bit for
+ * not see do not reach its output, whatever they hold. workspace: ..._workspace_size() bytes (0: none), 16-byte
+ * aligned, written before it is read; calls that may run at the same time need one each. No atomics: results repeat bit for
  * bit on one device. */
 size_t camblas_cuda_paged_decode_workspace_size(const camblas_cuda_context *context, int batch, int q_heads,
                                                 const camblas_cuda_paged_cache *cache, int table_columns, int window,
@@ -438,9 +439,9 @@ int camblas_cuda_paged_decode_attention(camblas_cuda_context *context, int batch
 size_t camblas_cuda_paged_prefill_workspace_size(const camblas_cuda_context *context, int batch, int tokens, int q_heads,
                                                  const camblas_cuda_paged_cache *cache, int table_columns, int window,
                                                  int sinks);
-/* The new tokens of ragged sequences, causal: rows query_starts[b] .. query_starts[b + 1] - 1 of q (int32 [batch + 1] on
- * the device, ascending, at most `tokens`) are sequence b's, the last of them at position lengths[b] - 1; each sees the positions up
- * to its own (or the window and the first tokens, as above). Rows that belong to no sequence are left
+/* The new tokens of ragged sequences, causal: rows query_starts[b] .. query_starts[b + 1] - 1 of q (int32
+ * [batch + 1] on the device, ascending, at most `tokens`) are sequence b's, the last of them at position
+ * lengths[b] - 1; each sees the positions up to its own (or the window and the first tokens, as above). Rows that belong to no sequence are left
  * as they were. The rest, the workspace with its own size among it, as above. */
 int camblas_cuda_paged_prefill_attention(camblas_cuda_context *context, int batch, int tokens, int q_heads,
                                          const camblas_cuda_paged_cache *cache, const int32_t *page_table,

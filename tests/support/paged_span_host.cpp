@@ -44,3 +44,9 @@ extern "C" int find_length(int32_t length, int columns, int page_shift)
 extern "C" int64_t find_share_begin(int64_t all, int64_t workers, int64_t g) { return share_begin(all, workers, g); }
 extern "C" int64_t find_share(int64_t all, int64_t workers, int64_t step) { return share_of(all, workers, step); }
 extern "C" int find_first_block(int token, int group, int rows, int sequence) { return first_block(token, group, rows, sequence); }
+extern "C" int find_apart(int64_t a, int64_t a_count, int64_t a_width, int64_t a_stride, int64_t b, int64_t b_count, int64_t b_width,
+                          int64_t b_stride)
+{
+    const auto *memory = reinterpret_cast<const unsigned short *>(uintptr_t(1) << 40);
+    return rows_apart(Rows{memory + a, a_count, a_width, a_stride}, Rows{memory + b, b_count, b_width, b_stride});
+}

@@ -113,6 +113,26 @@ def test_numbers_of_row_blocks(host):
         assert first[-1] == starts[-1] * group // rows + len(counts) and all(n < first[-1] for n in used)
 
 
+def test_rows_that_share_memory(host):
+    rng = random.Random(4)
+    host.find_apart.argtypes = [ct.c_int64] * 8
+    seen = set()
+    for _ in range(3000):
+        stride = rng.choice([4, 8, 12])
+        a, b = ([rng.randint(0, 30), rng.randint(0, 3), rng.randint(1, 6), rng.choice([stride, stride, stride, 5])] for _ in range(2))
+        cells = [{x[0] + r * x[3] + i for r in range(x[1]) for i in range(x[2])} for x in (a, b)]
+        apart = bool(host.find_apart(*a, *b))
+        if apart:
+            assert not cells[0] & cells[1]
+        elif a[3] == b[3] and a[2] <= stride and b[2] <= stride and a[1] > 1 and b[1] > 1 and a[1] == b[1]:
+            # rows of one stride that are refused share an element, at least were both to go on
+            go_on = [{x[0] + r * x[3] + i for r in range(-12, 12) for i in range(x[2])} for x in (a, b)]
+            assert go_on[0] & go_on[1]
+        seen.add(apart)
+    assert seen == {True, False}
+    assert host.find_apart(0, 5, 8, 24, 8, 5, 8, 24) and not host.find_apart(0, 5, 8, 24, 7, 5, 8, 24)
+
+
 def test_tensors_without_a_gpu_are_refused():
     q, cache = torch.zeros(2, 4, 64, dtype=torch.bfloat16), torch.zeros(3, 16, 2, 64, dtype=torch.bfloat16)
     table, lengths = torch.zeros(2, 2, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)

@@ -366,6 +366,45 @@ def test_empty_batches(device):
     assert not _kernels.paged_decode_attention(q, k, v, table[:1, :0].expand(2, 0).contiguous(), held).any()
 
 
+def test_axes_of_one_element_and_shared_table_rows(device):
+    # strides of axes of one element are anything; a table row may serve several sequences
+    k, v, table = reference.paged_case(2550, [50], page_size=64, kv_heads=1, dim=64, device=device, spare=0)
+    odd = [torch.as_strided(t.clone(), t.shape, (7, 64, 3, 1)) for t in (k, v)]
+    q = queries(2551, 3, 4, 64, device)
+    held = torch.tensor([50, 7, 33], dtype=torch.int32, device=device)
+    rows = table[:1].expand(3, table.shape[1])
+    got = _kernels.paged_decode_attention(q, *odd, rows, held)
+    want, allowed = reference.attention_rows(q, k, v, rows, [50, 7, 33], [1, 1, 1])
+    assert reference.within(got, want, allowed)
+    one = torch.as_strided(q, (1, 4, 64), (5, 64, 1))
+    starts = torch.tensor([0, 1], dtype=torch.int32, device=device)
+    got = _kernels.paged_prefill_attention(one, *odd, rows[:1], held[:1], starts)
+    assert reference.within(got, want[:1], allowed[:1])
+
+
+def test_starts_out_of_order_write_only_rows_of_sequences(device):
+    k, v, table = reference.paged_case(2560, [20, 20], page_size=16, kv_heads=1, dim=64, device=device)
+    q = queries(2561, 9, 4, 64, device)
+    held = torch.tensor([20, 20], dtype=torch.int32, device=device)
+    out = torch.full_like(q, 3.0)
+    starts = torch.tensor([5, 2, 1000], dtype=torch.int32, device=device)  # the first has none, the second rows 2 to 8
+    _kernels.paged_prefill_attention(q, k, v, table, held, starts, out=out)
+    want, allowed = reference.attention_rows(q[2:], k, v, table[1:], [20], [7])
+    assert (out[:2] == 3).all() and reference.within(out[2:], want, allowed)
+
+
+def test_starts_in_no_order_stay_inside(device):
+    batch, tokens = 600, 70
+    k, v, table = reference.paged_case(2570, [30] * batch, page_size=16, kv_heads=2, dim=64, device=device)
+    room = torch.full((tokens + 40, 4, 64), 3.0, dtype=torch.bfloat16, device=device)
+    q = queries(2571, tokens, 4, 64, device)
+    generator = torch.Generator().manual_seed(2572)
+    starts = torch.randint(-50, 200, (batch + 1,), generator=generator, dtype=torch.int32).to(device)
+    held = torch.full((batch,), 30, dtype=torch.int32, device=device)
+    _kernels.paged_prefill_attention(q, k, v, table, held, starts, out=room[20:-20])
+    assert (room[:20] == 3).all() and (room[-20:] == 3).all() and torch.isfinite(room).all()
+
+
 def refused(call, *arguments, **options):
     with pytest.raises((RuntimeError, ValueError, TypeError)):
         call(*arguments, **options)
@@ -396,6 +435,10 @@ def test_refusals(device):
     refused(decode, q, k, v, table, held, window=-1)
     refused(decode, q, k, v, table, held, sinks=-1)
     refused(decode, q, k, v, table, held, out=q)
+    wide = queries(2603, 2, 20, 128, device)
+    decode(wide[:, :8], k, v, table, held, out=wide[:, 12:])          # heads of one activation beside each other
+    refused(decode, wide[:, :8], k, v, table, held, out=wide[:, 6:14])  # and on each other
+    refused(decode, q, k, v, table, held, out=k.flatten()[: q.numel()].view_as(q))  # into the cache
     refused(decode, q.clone().requires_grad_(), k, v, table, held)
     starts = torch.tensor([0, 1, 2], dtype=torch.int32, device=device)
     prefill = _kernels.paged_prefill_attention
@@ -422,6 +465,8 @@ def test_refusals(device):
     for theta in (0.0, -5.0, math.nan):
         refused(append, qkv, position, slots, k, v, theta=theta, **options)
     refused(append, qkv, position, slots, k, v, epsilon=-1.0, **options)
+    refused(append, qkv, position, slots, k, v, out=qkv[:, 1:9], **options)
+    refused(append, k.flatten()[: qkv.numel()].view_as(qkv), position, slots, k, v, **options)
     refused(append, qkv, position, slots, k, v, out=torch.empty(2, 7, 128, dtype=torch.bfloat16, device=device), **options)
 
 
