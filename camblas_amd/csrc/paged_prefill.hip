@@ -432,19 +432,21 @@ template <int DIM, bool SHARED> __global__ __launch_bounds__(THREADS, DIM == 64 
             }
         // The order asked of the compiler: every matrix instruction is followed by vector instructions that fill
         // its 32 cycles and by the reads of an operand to come (left alone it put the products of the scores in a
-        // row: 2264 against 2177 us at 2048 tokens after 30001).
+        // row: 2264 against 2177 us at 2048 tokens after 30001, heads of 128). Heads of 64 have half the matrix
+        // instructions for as many of the others: 10 and 4 of them after each took 161 us where 5 and 2 took 169.
+        constexpr int AFTER_SCORES = DIM == 64 ? 10 : 5, AFTER_VALUES = DIM == 64 ? 4 : 2;
         __builtin_amdgcn_sched_group_barrier(DS_READS, 4, 0);
 #pragma unroll
         for (int i = 0; i < 2 * DIM / 16; ++i) {
             __builtin_amdgcn_sched_group_barrier(MATRIX, 1, 0);
             __builtin_amdgcn_sched_group_barrier(DS_READS, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(VECTOR, 5, 0);
+            __builtin_amdgcn_sched_group_barrier(VECTOR, AFTER_SCORES, 0);
         }
 #pragma unroll
         for (int i = 0; i < TILE / 16 * DIM / 32; ++i) {
             __builtin_amdgcn_sched_group_barrier(MATRIX, 1, 0);
             __builtin_amdgcn_sched_group_barrier(DS_READS, 2, 0);
-            __builtin_amdgcn_sched_group_barrier(VECTOR, 2, 0);
+            __builtin_amdgcn_sched_group_barrier(VECTOR, AFTER_VALUES, 0);
         }
         wanted = next_wanted;
         asm volatile("" ::: "memory");
@@ -524,35 +526,50 @@ template <int DIM, bool SHARED> __global__ __launch_bounds__(THREADS, DIM == 64 
     }
 }
 
-// Joins the shares of the rows of a block in their order; DIM / 4 threads take a row, and a workgroup as many rows
-// as it has threads for (four rows after each other made 16 us of it where one makes 5).
-template <int DIM> constexpr int join_rows() { return THREADS / (DIM / 4); }
+// Joins the shares of a token's heads in their order; DIM / 4 threads take a head. What the shares left is on its way
+// while the starts tell whether the token is any sequence's (finding the block first cost a trip to memory of its own).
+template <int DIM> constexpr int join_heads() { return THREADS / (DIM / 4); }
 template <int DIM> __global__ __launch_bounds__(THREADS) void paged_prefill_join_kernel(PrefillParams p)
 {
-    constexpr int ROW = DIM / 4;
-    Block block;
-    if (!find_block(p, blockIdx.x, block))
-        return;
-    const int r = int(blockIdx.y * join_rows<DIM>() + threadIdx.x / ROW);
-    if (r >= block.rows)
-        return;
-    const int d = 4 * (threadIdx.x % ROW), q_heads = p.cache.kv_heads * p.group;
-    const unsigned row = unsigned(block.row0 + r), group = p.group;
-    const int token = block.token0 + int(row / group), head = block.kv_head * p.group + int(row % group);
-    const size_t first = size_t(token) * q_heads + head, step = size_t(p.tokens) * q_heads;
-    float top = -INFINITY;
-#pragma unroll 4
-    for (int s = 0; s < p.shares; ++s)
-        top = fmaxf(top, p.part_m[first + s * step]);
-    const float reference = top == -INFINITY ? 0.f : top;
+    constexpr int ROW = DIM / 4, HEADS = join_heads<DIM>(), AT_ONCE = 8; // shares on their way together
+    const int q_heads = p.cache.kv_heads * p.group, parts = (q_heads + HEADS - 1) / HEADS;
+    const int token = blockIdx.x / parts, head = blockIdx.x % parts * HEADS + threadIdx.x / ROW;
+    const int d = 4 * (threadIdx.x % ROW);
+    const size_t first = size_t(token) * q_heads + min(head, q_heads - 1), step = size_t(p.tokens) * q_heads;
+    bool owned = false;
+    for (int b = threadIdx.x; b < p.batch; b += THREADS)
+        owned = owned || (first_token(p, b) <= token && token < first_token(p, b + 1));
+    float top = -INFINITY, sum = 0.f;
     f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-    float sum = 0.f;
-#pragma unroll 4
-    for (int s = 0; s < p.shares; ++s) {
-        const float factor = __builtin_amdgcn_exp2f(p.part_m[first + s * step] - reference);
-        sum = fmaf(factor, p.part_l[first + s * step], sum);
-        o += factor * *reinterpret_cast<const f32x4_t *>(p.part_o + (first + s * step) * DIM + d);
+    for (int share = 0; share < p.shares; share += AT_ONCE) {
+        float m[AT_ONCE], l[AT_ONCE];
+        f32x4_t part[AT_ONCE];
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) {
+            const size_t at = first + size_t(min(share + i, p.shares - 1)) * step;
+            m[i] = p.part_m[at];
+            l[i] = p.part_l[at];
+            part[i] = *reinterpret_cast<const f32x4_t *>(p.part_o + at * DIM + d);
+        }
+        if (share == 0 && !__syncthreads_or(owned))
+            return;
+        const float before = top;
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i)
+            top = fmaxf(top, m[i]);
+        const float reference = top == -INFINITY ? 0.f : top, kept = __builtin_amdgcn_exp2f(before - reference);
+        sum *= kept;
+        o *= kept;
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i)
+            if (share + i < p.shares) {
+                const float factor = __builtin_amdgcn_exp2f(m[i] - reference);
+                sum = fmaf(factor, l[i], sum);
+                o += factor * part[i];
+            }
     }
+    if (head >= q_heads)
+        return;
     o *= sum == 0.f ? 0.f : 1.f / sum;
     *reinterpret_cast<u32x2_t *>(p.out + int64_t(token) * p.out_stride + int64_t(head) * DIM + d) =
         u32x2_t{round_pair(o[0], o[1]), round_pair(o[2], o[3])};
@@ -628,7 +645,8 @@ hipError_t launch_paged_prefill(hipStream_t stream, int batch, int tokens, int q
     if (status != hipSuccess)
         return status;
     const auto join = dim == 128 ? paged_prefill_join_kernel<128> : paged_prefill_join_kernel<64>;
-    join<<<dim3(numbers, ROWS / (dim == 128 ? join_rows<128>() : join_rows<64>())), THREADS, 0, stream>>>(p);
+    const int heads = dim == 128 ? join_heads<128>() : join_heads<64>();
+    join<<<unsigned(tokens) * ((q_heads + heads - 1) / heads), THREADS, 0, stream>>>(p);
     return launch_status();
 }
 } // namespace camblas_hip

@@ -393,6 +393,20 @@ def test_starts_out_of_order_write_only_rows_of_sequences(device):
     assert (out[:2] == 3).all() and reference.within(out[2:], want, allowed)
 
 
+@pytest.mark.parametrize("q_heads, kv_heads, dim", [(5, 1, 128), (6, 2, 64), (40, 2, 128)])
+def test_shares_of_a_long_past_join_for_rows_of_sequences_only(q_heads, kv_heads, dim, device):
+    # positions divided over more workgroups than are joined at once; rows before, between and behind the sequences
+    k, v, table = reference.paged_case(2580, [9001, 17], page_size=16, kv_heads=kv_heads, dim=dim, device=device)
+    q = queries(2581, 9, q_heads, dim, device)
+    held = torch.tensor([9001, 17], dtype=torch.int32, device=device)
+    out = torch.full_like(q, 3.0)
+    starts = torch.tensor([2, 5, 6], dtype=torch.int32, device=device)
+    _kernels.paged_prefill_attention(q, k, v, table, held, starts, out=out)
+    want, allowed = reference.attention_rows(q[2:6], k, v, table, [9001, 17], [3, 1])
+    assert (out[:2] == 3).all() and (out[6:] == 3).all()
+    assert reference.within(out[2:6], want, allowed)
+
+
 def test_starts_in_no_order_stay_inside(device):
     batch, tokens = 600, 70
     k, v, table = reference.paged_case(2570, [30] * batch, page_size=16, kv_heads=2, dim=64, device=device)
