@@ -790,7 +790,7 @@ def _tensor_binding():
 
 
 # The paged cache's operators go through the tensor binding: a decode step's kernels take a few microseconds,
-# less than checking and passing a dozen arguments through ctypes (16 against 5 us a call).
+# less than checking and passing a dozen arguments through ctypes (16 against 4 us a call).
 
 
 def qk_norm_rope_append(qkv, positions, slots, k_cache, v_cache, *, q_heads, kv_heads, q_weight=None, k_weight=None,
@@ -807,8 +807,7 @@ def qk_norm_rope_append(qkv, positions, slots, k_cache, v_cache, *, q_heads, kv_
     kv_heads, dim] tensor). `out` may be qkv[:, :q_heads].
     """
     return _tensor_binding().qk_norm_rope_append(
-        qkv, positions, slots, k_cache, v_cache, q_heads=q_heads, kv_heads=kv_heads, q_weight=q_weight, k_weight=k_weight,
-        epsilon=epsilon, theta=theta, rotary_dim=rotary_dim, out=out)
+        qkv, positions, slots, k_cache, v_cache, q_heads, kv_heads, q_weight, k_weight, epsilon, theta, rotary_dim, out)
 
 
 def paged_decode_attention(q, k_cache, v_cache, page_table, lengths, *, scale=None, window=0, sinks=0, out=None):
@@ -816,8 +815,7 @@ def paged_decode_attention(q, k_cache, v_cache, page_table, lengths, *, scale=No
     kv_heads, dim] found through page_table (int32 [batch, columns]; entries that are no page hold nothing); lengths
     (int32 [batch]) counts the positions of each sequence, the new token's among them. window > 0: only the last
     `window` positions and the first `sinks` are seen. BF16 [batch, q_heads, dim]; zeros where nothing is seen."""
-    return _tensor_binding().paged_decode_attention(q, k_cache, v_cache, page_table, lengths, scale=scale, window=window,
-                                                    sinks=sinks, out=out)
+    return _tensor_binding().paged_decode_attention(q, k_cache, v_cache, page_table, lengths, scale, window, sinks, out)
 
 
 def paged_prefill_attention(q, k_cache, v_cache, page_table, lengths, query_starts, *, scale=None, window=0, sinks=0, out=None):
@@ -826,8 +824,8 @@ def paged_prefill_attention(q, k_cache, v_cache, page_table, lengths, query_star
     query_starts[b + 1] - 1 (int32 [batch + 1]), the last of them at position lengths[b] - 1. The rest as
     paged_decode_attention; rows that belong to no sequence are left as they were (unset where `out` is made
     here)."""
-    return _tensor_binding().paged_prefill_attention(q, k_cache, v_cache, page_table, lengths, query_starts, scale=scale,
-                                                     window=window, sinks=sinks, out=out)
+    return _tensor_binding().paged_prefill_attention(q, k_cache, v_cache, page_table, lengths, query_starts, scale, window,
+                                                     sinks, out)
 
 
 def decoder_layer_decode(hidden, residual, weights, k_cache, v_cache, positions, lengths, *,

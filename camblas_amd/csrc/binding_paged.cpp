@@ -181,16 +181,17 @@ Tensor prefill(const Tensor &q, const Tensor &k_cache, const Tensor &v_cache, co
 
 void register_paged(py::module_ &module)
 {
+    // (by position too: eight arguments found by their names are 1 of 5 us of a call)
     module.def("qk_norm_rope_append", &append, py::arg("qkv"), py::arg("positions"), py::arg("slots"), py::arg("k_cache"),
-               py::arg("v_cache"), py::kw_only(), py::arg("q_heads"), py::arg("kv_heads"), py::arg("q_weight") = py::none(),
+               py::arg("v_cache"), py::arg("q_heads"), py::arg("kv_heads"), py::arg("q_weight") = py::none(),
                py::arg("k_weight") = py::none(), py::arg("epsilon") = 1e-6, py::arg("theta") = 500000.,
                py::arg("rotary_dim") = py::none(), py::arg("out") = py::none(),
                "Normalise and rotate query and key heads, append keys and values to a paged cache; the queries.");
     module.def("paged_decode_attention", &decode, py::arg("q"), py::arg("k_cache"), py::arg("v_cache"), py::arg("page_table"),
-               py::arg("lengths"), py::kw_only(), py::arg("scale") = py::none(), py::arg("window") = 0, py::arg("sinks") = 0,
+               py::arg("lengths"), py::arg("scale") = py::none(), py::arg("window") = 0, py::arg("sinks") = 0,
                py::arg("out") = py::none(), "Attention of one new token per sequence over a paged cache.");
     module.def("paged_prefill_attention", &prefill, py::arg("q"), py::arg("k_cache"), py::arg("v_cache"),
-               py::arg("page_table"), py::arg("lengths"), py::arg("query_starts"), py::kw_only(),
+               py::arg("page_table"), py::arg("lengths"), py::arg("query_starts"),
                py::arg("scale") = py::none(), py::arg("window") = 0, py::arg("sinks") = 0, py::arg("out") = py::none(),
                "Causal attention of the new tokens of ragged sequences over a paged cache.");
 }
