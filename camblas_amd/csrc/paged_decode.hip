@@ -13,9 +13,9 @@
 // the maximum that weights refer to is moved only when a score exceeds it by 2^8, so that the outputs are
 // rarely rescaled; weights are rounded to BF16 for the second product, their sum is kept in FP32.
 //
-// Measured, 64 query and 8 key-value heads of 128: 32 sequences of 2048 positions 46 us, 5.9 TB/s; 64 of 1 to
-// 16384 382 us, 6.0 TB/s; one of 131072 98 us, 5.5 TB/s (a copy of 2 GiB moves 4.9 TB/s, reads alone
-// are faster). Small calls are bound by their trips to memory, one after the other: length and page, K, V.
+// Measured, 64 query and 8 key-value heads of 128: 32 sequences of 2048 positions 44.5 us, 6.05 TB/s; 64 of 1 to
+// 16384 378 us, 6.0 TB/s; one of 131072 96 us, 5.6 TB/s (a copy of 2 GiB moves 4.9 TB/s, reads alone are faster);
+// one of 129 5.2 us. Small calls are bound by their trips to memory, one after the other: length and page, K and V.
 //
 // Work is divided by what the sequences hold, not by what the table could hold: all steps of a tile for each
 // wavefront (sequence, key-value head and 16 query heads, positions) are numbered and every workgroup takes an equal
@@ -283,26 +283,29 @@ __device__ __forceinline__ void work_item(const DecodeParams &p, const unsigned 
             *reinterpret_cast<f32x4_t *>(&wave_o[wave][m][(DIM / 16) * (4 * j + r) + w]) =
                 f32x4_t{run.acc[w][r], run.acc[w + 1][r], run.acc[w + 2][r], run.acc[w + 3][r]};
     __syncthreads();
-    for (int index = thread; index < item.heads * DIM; index += WAVES * 64) {
-        const int h = index / DIM, d = index % DIM;
+    // (four dims a thread, one piece to memory: one by one they made 129 positions 5.9 us of 5.2)
+    for (int index = thread; index < item.heads * DIM / 4; index += WAVES * 64) {
+        const int h = index / (DIM / 4), d = 4 * (index % (DIM / 4));
         float best = wave_m[0][h];
 #pragma unroll
         for (int w = 1; w < WAVES; ++w)
             best = fmaxf(best, wave_m[w][h]);
         const float reference = best == -INFINITY ? 0.f : best;
-        float numerator = 0.f, denominator = 0.f;
+        f32x4_t numerator = {0.f, 0.f, 0.f, 0.f};
+        float denominator = 0.f;
 #pragma unroll
         for (int w = 0; w < WAVES; ++w) {
-            const float factor = exp2f(wave_m[w][h] - reference);
-            numerator = fmaf(factor, wave_o[w][h][d], numerator);
+            const float factor = __builtin_amdgcn_exp2f(wave_m[w][h] - reference);
+            numerator += factor * *reinterpret_cast<const f32x4_t *>(&wave_o[w][h][d]);
             denominator = fmaf(factor, wave_l[w][h], denominator);
         }
         if (slot < 0) {
             // (no position seen: zero; a sum that is NaN stays NaN)
-            p.out[int64_t(item.sequence) * p.out_stride + int64_t(item.head0 + h) * DIM + d] =
-                float_to_bf16_bits(denominator == 0.f ? 0.f : numerator / denominator);
+            numerator *= denominator == 0.f ? 0.f : 1.f / denominator;
+            *reinterpret_cast<u32x2_t *>(p.out + int64_t(item.sequence) * p.out_stride + int64_t(item.head0 + h) * DIM + d) =
+                u32x2_t{round_pair(numerator[0], numerator[1]), round_pair(numerator[2], numerator[3])};
         } else {
-            p.part_o[(size_t(slot) * HEADS + h) * DIM + d] = numerator;
+            *reinterpret_cast<f32x4_t *>(p.part_o + (size_t(slot) * HEADS + h) * DIM + d) = numerator;
             if (d == 0) {
                 p.part_m[slot * HEADS + h] = best;
                 p.part_l[slot * HEADS + h] = denominator;
@@ -428,16 +431,18 @@ template <int DIM, bool LARGE> __global__ __launch_bounds__(SHARE_WAVES * 64, 2)
 }
 
 // Joins the partials of one query head in the order of its positions; zeros where the sequence holds
-// nothing. A head that a single workgroup held is written already. All maxima are read at once, then DIM / 4
-// threads take a partial's row and the rows are dealt to the groups of threads: two trips to memory and an
-// ordered sum, whatever the number of partials (one thread per dim walking 64 of them took 140 us).
+// nothing. A head that a single workgroup held is written already. DIM / 4 threads take a partial's row and the
+// rows are dealt to the groups of threads: an ordered sum, whatever the number of partials (one thread per dim
+// walking 64 of them took 140 us). Two trips to memory: what says where the partials lie, and all of them, up to
+// AHEAD rows a group (maxima, sums and rows one after the other made five: 131072 positions 97.2 / 96.0 us).
 template <int DIM> __global__ __launch_bounds__(JOIN_THREADS) void paged_decode_join_kernel(DecodeParams p)
 {
-    constexpr int ROW = DIM / 4, GROUPS = JOIN_THREADS / ROW, JOIN_WAVES = JOIN_THREADS / 64;
+    constexpr int ROW = DIM / 4, GROUPS = JOIN_THREADS / ROW, JOIN_WAVES = JOIN_THREADS / 64, AHEAD = 8;
     __shared__ float weight[MOST_SHARES], group_o[GROUPS][DIM], wave_top[JOIN_WAVES], wave_sums[JOIN_WAVES];
     const int thread = threadIdx.x, lane = thread % 64, wave = thread / 64;
     const int head = blockIdx.x, sequence = blockIdx.y, items = p.cache.kv_heads * p.head_tiles;
     const int within = head % p.group, h = within % HEADS;
+    const int2 join = p.joins[size_t(sequence) * items + head / p.group * p.head_tiles + within / HEADS]; // (unset: not used)
     int query;
     const bool empty = span_of(p, sequence, query).tiles == 0;
     unsigned short *out = p.out + int64_t(sequence) * p.out_stride + int64_t(head) * DIM;
@@ -446,17 +451,23 @@ template <int DIM> __global__ __launch_bounds__(JOIN_THREADS) void paged_decode_
             out[thread] = 0;
         return;
     }
-    const int2 join = p.joins[size_t(sequence) * items + head / p.group * p.head_tiles + within / HEADS];
     const int count = join.y - join.x + 1;
     if (count == 1)
         return;
     const auto row_of = [&](int i) { return size_t(2 * (join.x + i) + (i == 0)) * HEADS + h; };
-    float top = -INFINITY;
-    for (int i = thread; i < count; i += JOIN_THREADS) {
-        const float m = p.part_m[row_of(i)];
-        weight[i] = m;
-        top = fmaxf(top, m);
-    }
+    const int group = thread / ROW, d = 4 * (thread % ROW);
+    const auto part = [&](int i) { return *reinterpret_cast<const f32x4_t *>(p.part_o + row_of(i) * DIM + d); };
+    // (threads without a partial read the last one)
+    const int own = min(thread, count - 1);
+    const float own_top = p.part_m[row_of(own)];
+    const float own_sum = p.part_l[row_of(own)];
+    f32x4_t ahead[AHEAD];
+#pragma unroll
+    for (int n = 0; n < AHEAD; ++n)
+        ahead[n] = part(min(group + n * GROUPS, count - 1));
+    float top = own_top;
+    for (int i = thread + JOIN_THREADS; i < count; i += JOIN_THREADS)
+        top = fmaxf(top, p.part_m[row_of(i)]);
     top = wave_max(top);
     if (lane == 0)
         wave_top[wave] = top;
@@ -466,21 +477,25 @@ template <int DIM> __global__ __launch_bounds__(JOIN_THREADS) void paged_decode_
     for (int w = 1; w < JOIN_WAVES; ++w)
         top = fmaxf(top, wave_top[w]);
     const float reference = top == -INFINITY ? 0.f : top;
-    float sum = 0.f;
-    for (int i = thread; i < count; i += JOIN_THREADS) {
-        const float factor = __builtin_amdgcn_exp2f(weight[i] - reference);
-        weight[i] = factor;
-        sum = fmaf(factor, p.part_l[row_of(i)], sum);
+    const float own_factor = __builtin_amdgcn_exp2f(own_top - reference);
+    float sum = thread < count ? own_factor * own_sum : 0.f;
+    weight[thread] = own_factor;
+    for (int i = thread + JOIN_THREADS; i < count; i += JOIN_THREADS) {
+        weight[i] = __builtin_amdgcn_exp2f(p.part_m[row_of(i)] - reference);
+        sum = fmaf(weight[i], p.part_l[row_of(i)], sum);
     }
     sum = wave_sum(sum);
     if (lane == 0)
         wave_sums[wave] = sum;
     __syncthreads();
-    const int group = thread / ROW, d = 4 * (thread % ROW);
     f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int n = 0; n < AHEAD; ++n)
+        if (group + n * GROUPS < count)
+            o += weight[group + n * GROUPS] * ahead[n];
 #pragma unroll 4
-    for (int i = group; i < count; i += GROUPS)
-        o += weight[i] * *reinterpret_cast<const f32x4_t *>(p.part_o + row_of(i) * DIM + d);
+    for (int i = group + AHEAD * GROUPS; i < count; i += GROUPS)
+        o += weight[i] * part(i);
     *reinterpret_cast<f32x4_t *>(&group_o[group][d]) = o;
     __syncthreads();
     if (thread < DIM) {
@@ -497,11 +512,11 @@ template <int DIM> __global__ __launch_bounds__(JOIN_THREADS) void paged_decode_
 } // namespace
 
 // How a call is divided: workgroups that share all steps, or 0 for one workgroup per (heads, sequence).
-// Sharing costs a second launch and the numbering of the steps, some 6 us, and keeps every compute unit busy
+// Sharing costs a second launch and the numbering of the steps, some 4 us, and keeps every compute unit busy
 // whatever the lengths; one workgroup each is done when the longest sequence is. Measured, 64 query and 8
-// key-value heads of 128, whole / shared: 8 items of 512 positions 11.7 / 12.3 us, of 1024 18 / 12; 128 items of
-// 1024 20 / 21, of 2048 35 / 32 (lengths from 1 to that 30 / 21); 256 items of 2048 46 / 53 (36 / 38), of 4096
-// 85 / 93 (64 / 52).
+// key-value heads of 128, whole / shared: 8 items of 512 positions 9.9 / 11.2 us, of 1024 15.4 / 11.2; 128 items of
+// 1024 17.9 / 20.2, of 2048 31.7 / 30.8 (lengths from 1 to that 25 / 20); 256 items of 2048 45 / 52 (35 / 37), of
+// 4096 84 / 93 (63 / 49).
 static int decode_shares(int64_t items, int64_t positions, int compute_units)
 {
     const int64_t busy = items < compute_units ? items : compute_units;
