@@ -226,6 +226,9 @@ template <int DIM, bool SHARED> __global__ __launch_bounds__(THREADS, DIM == 64 
 
     // which rows of the tile at hand exist and are seen by some query of the block
     uint64_t wanted = 0;
+    // Few new tokens leave wavefronts without a row: those only fetch (16 tokens past 1000 positions each 23.9 / 22.0 us, 4
+    // times 100 past 4000 53.4 / 51.5; heads of 64 have no registers left for it).
+    const bool works = !SHARED || DIM == 64 || wave * 32 < rows;
     // bit n: the lane's query sees position base + n
     const auto seen_rows = [&](int base) {
         uint64_t seen = wanted & below(query - base + 1);
@@ -333,14 +336,15 @@ template <int DIM, bool SHARED> __global__ __launch_bounds__(THREADS, DIM == 64 
         uint64_t rows_infinite = 0;
         if (!whole) { // (the same in every wavefront)
             const uint64_t own = seen_rows(base) >> (4 * half);
+            if (works)
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+                for (int t = 0; t < 2; ++t)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    // (all bits of a lane's own bit, and a bitwise choice: no masks in scalar registers)
-                    const int keep = __builtin_amdgcn_sbfe(int(own >> (32 * t)), 8 * (r / 4) + r % 4, 1);
-                    score[t][r] = __int_as_float((__float_as_int(score[t][r]) & keep) | (int(0xff800000u) & ~keep));
-                }
+                    for (int r = 0; r < 16; ++r) {
+                        // (all bits of a lane's own bit, and a bitwise choice: no masks in scalar registers)
+                        const int keep = __builtin_amdgcn_sbfe(int(own >> (32 * t)), 8 * (r / 4) + r % 4, 1);
+                        score[t][r] = __int_as_float((__float_as_int(score[t][r]) & keep) | (int(0xff800000u) & ~keep));
+                    }
             // A weight of zero times NaN or infinity would reach the output. Rows that nobody sees become zeros. A
             // row that some see and that holds such values has them taken out of the product and added, as they
             // are, to the sums of those who see it: no weight changes what becomes of those.
@@ -355,26 +359,28 @@ template <int DIM, bool SHARED> __global__ __launch_bounds__(THREADS, DIM == 64 
             __syncthreads();
             rows_infinite = uint64_t(unsigned(uniform(int(infinite[0])))) | uint64_t(unsigned(uniform(int(infinite[1])))) << 32;
         }
-        float highest = -INFINITY;
+        if (works) {
+            float highest = -INFINITY;
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+            for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int r = 0; r < 16; ++r)
-                highest = fmaxf(highest, score[t][r]);
-        highest *= p.scale;
-        if (__any(highest > top + 8.f)) {
-            highest = fmaxf(highest, __shfl_xor(highest, 32));
-            highest = fmaxf(highest, top);
-            const float factor = top == highest ? 1.f : __builtin_amdgcn_exp2f(top - highest);
-            top = highest;
-            total *= factor;
+                for (int r = 0; r < 16; ++r)
+                    highest = fmaxf(highest, score[t][r]);
+            highest *= p.scale;
+            if (__any(highest > top + 8.f)) {
+                highest = fmaxf(highest, __shfl_xor(highest, 32));
+                highest = fmaxf(highest, top);
+                const float factor = top == highest ? 1.f : __builtin_amdgcn_exp2f(top - highest);
+                top = highest;
+                total *= factor;
 #pragma unroll
-            for (int d = 0; d < DIM / 32; ++d)
-                acc[d] *= factor;
+                for (int d = 0; d < DIM / 32; ++d)
+                    acc[d] *= factor;
+            }
         }
         if (rows_infinite) {
             const uint64_t seen = seen_rows(base);
-            for (uint64_t left = rows_infinite; left; left &= left - 1) {
+            for (uint64_t left = works ? rows_infinite : 0; left; left &= left - 1) {
                 const int r = __builtin_ctzll(left);
                 const bool sees_it = (seen >> r) & 1;
 #pragma unroll
@@ -403,51 +409,53 @@ template <int DIM, bool SHARED> __global__ __launch_bounds__(THREADS, DIM == 64 
                 infinite[thread] = 0;
             __syncthreads();
         }
-        const float reference = top == -INFINITY ? 0.f : top;
-        multiply_keys(next_keys, next_score);
-        bf16x8_t weights[4];
+        if (works) {
+            const float reference = top == -INFINITY ? 0.f : top;
+            multiply_keys(next_keys, next_score);
+            bf16x8_t weights[4];
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
+            for (int t = 0; t < 2; ++t) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                score[t][r] = __builtin_amdgcn_exp2f(fmaf(score[t][r], p.scale, -reference));
-                total += score[t][r];
+                for (int r = 0; r < 16; ++r) {
+                    score[t][r] = __builtin_amdgcn_exp2f(fmaf(score[t][r], p.scale, -reference));
+                    total += score[t][r];
+                }
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+                    weights[2 * t + u] = __builtin_bit_cast(
+                        bf16x8_t, u32x4_t{round_pair(score[t][8 * u], score[t][8 * u + 1]),
+                                          round_pair(score[t][8 * u + 2], score[t][8 * u + 3]),
+                                          round_pair(score[t][8 * u + 4], score[t][8 * u + 5]),
+                                          round_pair(score[t][8 * u + 6], score[t][8 * u + 7])});
             }
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
-                weights[2 * t + u] = __builtin_bit_cast(
-                    bf16x8_t, u32x4_t{round_pair(score[t][8 * u], score[t][8 * u + 1]),
-                                      round_pair(score[t][8 * u + 2], score[t][8 * u + 3]),
-                                      round_pair(score[t][8 * u + 4], score[t][8 * u + 5]),
-                                      round_pair(score[t][8 * u + 6], score[t][8 * u + 7])});
-        }
+            for (int u = 0; u < TILE / 16; ++u)
 #pragma unroll
-        for (int u = 0; u < TILE / 16; ++u)
+                for (int d = 0; d < DIM / 32; ++d) {
+                    const i16x4_t lower = gather_column(values + value_at[d] + 16 * u * DIM * 2);
+                    const i16x4_t upper = gather_column(values + value_at[d] + (16 * u + 8) * DIM * 2);
+                    const bf16x8_t v = __builtin_bit_cast(
+                        bf16x8_t, i16x8_t{lower[0], lower[1], lower[2], lower[3], upper[0], upper[1], upper[2], upper[3]});
+                    acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, weights[u], acc[d], 0, 0, 0);
+                }
+            // The order asked of the compiler: every matrix instruction is followed by vector instructions that fill
+            // its 32 cycles and by the reads of an operand to come (left alone it put the products of the scores in a
+            // row: 2264 against 2177 us at 2048 tokens after 30001, heads of 128). Heads of 64 have half the matrix
+            // instructions for as many of the others: 10 and 4 of them after each took 161 us where 5 and 2 took 169.
+            constexpr int AFTER_SCORES = DIM == 64 ? 10 : 5, AFTER_VALUES = DIM == 64 ? 4 : 2;
+            __builtin_amdgcn_sched_group_barrier(DS_READS, 4, 0);
 #pragma unroll
-            for (int d = 0; d < DIM / 32; ++d) {
-                const i16x4_t lower = gather_column(values + value_at[d] + 16 * u * DIM * 2);
-                const i16x4_t upper = gather_column(values + value_at[d] + (16 * u + 8) * DIM * 2);
-                const bf16x8_t v = __builtin_bit_cast(
-                    bf16x8_t, i16x8_t{lower[0], lower[1], lower[2], lower[3], upper[0], upper[1], upper[2], upper[3]});
-                acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, weights[u], acc[d], 0, 0, 0);
+            for (int i = 0; i < 2 * DIM / 16; ++i) {
+                __builtin_amdgcn_sched_group_barrier(MATRIX, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(DS_READS, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(VECTOR, AFTER_SCORES, 0);
             }
-        // The order asked of the compiler: every matrix instruction is followed by vector instructions that fill
-        // its 32 cycles and by the reads of an operand to come (left alone it put the products of the scores in a
-        // row: 2264 against 2177 us at 2048 tokens after 30001, heads of 128). Heads of 64 have half the matrix
-        // instructions for as many of the others: 10 and 4 of them after each took 161 us where 5 and 2 took 169.
-        constexpr int AFTER_SCORES = DIM == 64 ? 10 : 5, AFTER_VALUES = DIM == 64 ? 4 : 2;
-        __builtin_amdgcn_sched_group_barrier(DS_READS, 4, 0);
 #pragma unroll
-        for (int i = 0; i < 2 * DIM / 16; ++i) {
-            __builtin_amdgcn_sched_group_barrier(MATRIX, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(DS_READS, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(VECTOR, AFTER_SCORES, 0);
-        }
-#pragma unroll
-        for (int i = 0; i < TILE / 16 * DIM / 32; ++i) {
-            __builtin_amdgcn_sched_group_barrier(MATRIX, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(DS_READS, 2, 0);
-            __builtin_amdgcn_sched_group_barrier(VECTOR, AFTER_VALUES, 0);
+            for (int i = 0; i < TILE / 16 * DIM / 32; ++i) {
+                __builtin_amdgcn_sched_group_barrier(MATRIX, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(DS_READS, 2, 0);
+                __builtin_amdgcn_sched_group_barrier(VECTOR, AFTER_VALUES, 0);
+            }
         }
         wanted = next_wanted;
         asm volatile("" ::: "memory");

@@ -407,6 +407,21 @@ def test_shares_of_a_long_past_join_for_rows_of_sequences_only(q_heads, kv_heads
     assert reference.within(out[2:6], want, allowed)
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+def test_few_rows_over_a_long_past_with_values_that_are_not_numbers(dim, device):
+    # three tokens of two heads fill a part of one wavefront of a block; its neighbours take part in cleaning the tiles
+    past, new = 4001, 3
+    k, v, table = reference.paged_case(2590, [past + new], page_size=16, kv_heads=1, dim=dim, device=device)
+    q = queries(2591, new, 2, dim, device)
+    for position, (column, value) in {past + 1: (3, math.nan), past + 2: (4, math.inf), past - 3: (5, -math.inf)}.items():
+        v[int(table[0, position // 16]), position % 16, 0, column] = value
+    held, starts = (torch.tensor(x, dtype=torch.int32, device=device) for x in ([past + new], [0, new]))
+    got = _kernels.paged_prefill_attention(q, k, v, table, held, starts)
+    want, allowed = reference.attention_rows(q, k, v, table, [past + new], [new])
+    assert torch.isnan(want[:, :, 3]).any(1).tolist() == [False, True, True] and torch.isinf(want[:, :, 4]).any(1).tolist() == [False, False, True]
+    assert reference.within(got, want, allowed)
+
+
 def test_starts_in_no_order_stay_inside(device):
     batch, tokens = 600, 70
     k, v, table = reference.paged_case(2570, [30] * batch, page_size=16, kv_heads=2, dim=64, device=device)
