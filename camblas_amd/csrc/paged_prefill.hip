@@ -52,6 +52,7 @@ struct PrefillParams {
     float *part_o, *part_m, *part_l;
 };
 
+typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
 typedef short i16x4_t __attribute__((ext_vector_type(4)));
 typedef short i16x8_t __attribute__((ext_vector_type(8)));
 __device__ __forceinline__ i16x4_t gather_column(const unsigned char *address)
@@ -191,6 +192,7 @@ __device__ __forceinline__ bool find_block(const PrefillParams &p, int number, B
 // SHARED: blockIdx.y of `shares` workgroups takes its part of the tiles and leaves what it has for the join.
 template <int DIM, bool SHARED> __global__ __launch_bounds__(THREADS, DIM == 64 ? 3 : 2) void paged_prefill_kernel(PrefillParams p)
 {
+    constexpr bool AHEAD = DIM == 128; // the next tile's scores are multiplied while this one's weights are worked out
     constexpr int CHUNKS = DIM / 8, FETCH = 64 / CHUNKS, FETCHES = TILE / FETCH / WAVES; // rows of a load, a wavefront's loads
     __shared__ __attribute__((aligned(16))) unsigned char keys0[TILE * DIM * 2], keys1[TILE * DIM * 2];
     __shared__ __attribute__((aligned(16))) unsigned char values0[TILE * DIM * 2], values1[TILE * DIM * 2];
@@ -227,8 +229,8 @@ template <int DIM, bool SHARED> __global__ __launch_bounds__(THREADS, DIM == 64 
     // which rows of the tile at hand exist and are seen by some query of the block
     uint64_t wanted = 0;
     // Few new tokens leave wavefronts without a row: those only fetch (16 tokens past 1000 positions each 23.9 / 22.0 us, 4
-    // times 100 past 4000 53.4 / 51.5; heads of 64 have no registers left for it).
-    const bool works = !SHARED || DIM == 64 || wave * 32 < rows;
+    // times 100 past 4000 53.4 / 51.5).
+    const bool works = !SHARED || wave * 32 < rows;
     // bit n: the lane's query sees position base + n
     const auto seen_rows = [&](int base) {
         uint64_t seen = wanted & below(query - base + 1);
@@ -239,14 +241,17 @@ template <int DIM, bool SHARED> __global__ __launch_bounds__(THREADS, DIM == 64 
 
     // ---- fetching tiles: lane r of every wavefront knows the page of tile row r
     const int32_t *pages = p.table.pages + int64_t(sequence) * p.table.stride;
-    const auto page_at = [&](int tile) {
-        return tile < end ? page_of(p.cache, pages, p.table.columns, span.position(tile) + lane) : -1;
+    // (loaded a turn before it is looked at; a tile behind the last one: the last one's)
+    const auto column_of = [&](int tile) { return (span.position(min(tile, end - 1)) + lane) >> p.cache.page_shift; };
+    const auto load_page = [&](int tile) { return pages[min(column_of(tile), p.table.columns - 1)]; };
+    const auto checked = [&](int tile, int page) {
+        return (column_of(tile) < p.table.columns) & (unsigned(page) < unsigned(p.cache.pages)) ? page : -1;
     };
     // which rows of a tile exist and are seen by some query of the block
     const auto wanted_rows = [&](int tile, int page) {
-        const int position = span.position(tile) + lane;
-        return __ballot(page >= 0 && position <= last_query &&
-                        (p.see.window <= 0 || position > first_query - p.see.window || position < p.see.sinks));
+        const int position = span.position(min(tile, end - 1)) + lane;
+        return __ballot((page >= 0) & (position <= last_query) &
+                        ((p.see.window <= 0) | (position > first_query - p.see.window) | (position < p.see.sinks)));
     };
     // A wavefront brings rows 16 * wave .. + 15, FETCH of them with a load, in the order of their turned chunks. Where
     // pages hold at least 16 rows those lie in one page, at offsets that are the same for every tile.
@@ -263,7 +268,7 @@ template <int DIM, bool SHARED> __global__ __launch_bounds__(THREADS, DIM == 64 
     }
     // where the wavefront's first row of a tile lies (a row that does not exist: some row that does, and is not used)
     const auto place = [&](int tile, int page) {
-        return row_offset(p.cache, max(__builtin_amdgcn_readlane(page, own_row), 0), span.position(tile) + own_row) + head_at;
+        return row_offset(p.cache, max(__builtin_amdgcn_readlane(page, own_row), 0), span.position(min(tile, end - 1)) + own_row) + head_at;
     };
     const auto fetch = [&](const unsigned short *array, const unsigned (&from)[FETCHES], int64_t at, int tile, int page,
                            unsigned char *to) {
@@ -314,23 +319,43 @@ template <int DIM, bool SHARED> __global__ __launch_bounds__(THREADS, DIM == 64 
         for (int r = 0; r < 16; ++r)
             acc[d][r] = 0.f;
 
-    // Turn `tile`: its scores are in `score`, its values in `values`, the keys of the next tile in `next_keys`.
-    // Fetched meanwhile: the next tile's values, the keys of the one after. The next tile's scores are multiplied
-    // while this one's weights are worked out.
-    int page, next_page; // of the rows of the next tile and of the one after
-    int64_t at = 0;      // place() of the next tile
+    // Turn `tile`: its keys and values are in `keys` and `values`. Heads of 128 (AHEAD) have its scores in `score` already
+    // and multiply the next tile's, whose keys are in `next_keys`, into `next_score` while the weights are worked out:
+    // fetched meanwhile are the next tile's values and the keys of the one after. Heads of 64 multiply their scores now
+    // and fetch the next tile: three wavefronts of a SIMD fill each other's gaps, and the registers of a second set of
+    // scores are better spent (windowed prompts 159 / 154 us).
+    // Page numbers are loaded before the loads to LDS (a wait for them would be one for those too), looked at a turn
+    // later, and made into addresses in the shadow of the products (all at the start of a turn it took 1000 of
+    // 3400 cycles: 2048 tokens after 30001 2000 / 1898 us).
+    uint64_t wanted1 = 0, wanted2 = 0;  // of the next tile and the one after
+    int page1 = 0, page2 = 0, raw3 = 0; // their pages, and what the table holds for the one after those
+    int64_t at1 = 0, at2 = 0;           // their place()
     const auto turn = [&](int tile, f32x16_t (&score)[2], f32x16_t (&next_score)[2], unsigned char *keys,
                           const unsigned char *next_keys, unsigned char *values, unsigned char *next_values) {
         const int base = span.position(tile);
-        const uint64_t next_wanted = wanted_rows(tile + 1, page);
+        int page3 = checked(tile + 3, raw3);
+        asm volatile("" : "+v"(page3));
+        raw3 = load_page(tile + 4);
         if (tile + 1 < end)
-            fetch(p.cache.v, value_from, at, tile + 1, page, next_values);
-        page = next_page;
-        if (tile + 2 < end) {
-            at = place(tile + 2, page);
-            fetch(p.cache.k, key_from, at, tile + 2, page, keys);
+            fetch(p.cache.v, value_from, at1, tile + 1, page1, next_values);
+        if constexpr (AHEAD) {
+            if (tile + 2 < end)
+                fetch(p.cache.k, key_from, at2, tile + 2, page2, keys);
+        } else {
+            if (tile + 1 < end)
+                fetch(p.cache.k, key_from, at1, tile + 1, page1, const_cast<unsigned char *>(next_keys));
+            if (works)
+                multiply_keys(keys, score);
         }
-        next_page = page_at(tile + 3);
+        const auto look_ahead = [&]() {
+            wanted = wanted1;
+            wanted1 = wanted2;
+            page1 = page2;
+            at1 = at2;
+            page2 = page3;
+            wanted2 = wanted_rows(tile + 3, page2);
+            at2 = place(tile + 3, page2);
+        };
         const bool whole = wanted == ~uint64_t(0) && base + TILE - 1 <= first_query &&
                            (p.see.window <= 0 || base > last_query - p.see.window || base + TILE <= p.see.sinks);
         uint64_t rows_infinite = 0;
@@ -348,14 +373,30 @@ template <int DIM, bool SHARED> __global__ __launch_bounds__(THREADS, DIM == 64 
             // A weight of zero times NaN or infinity would reach the output. Rows that nobody sees become zeros. A
             // row that some see and that holds such values has them taken out of the product and added, as they
             // are, to the sums of those who see it: no weight changes what becomes of those.
-            for (int piece = thread; piece < TILE * CHUNKS; piece += THREADS) {
-                u32x4_t *at_piece = reinterpret_cast<u32x4_t *>(values + piece * 16);
-                const int r = piece / CHUNKS;
-                if (!((wanted >> r) & 1))
-                    *at_piece = u32x4_t{0, 0, 0, 0};
-                else if (holds_infinite(*at_piece))
-                    atomicOr(&infinite[r / 32], 1u << (r % 32));
+            constexpr int PIECES = TILE * CHUNKS / THREADS;
+            u32x4_t *own_pieces = reinterpret_cast<u32x4_t *>(values) + thread, piece[PIECES];
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i)
+                piece[i] = own_pieces[i * THREADS];
+            u16x2_t largest = {0, 0}; // of the bits without the sign: those of infinities and NaN are the largest
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) {
+                const int r = (thread + i * THREADS) / CHUNKS;
+                if (!((wanted >> r) & 1)) {
+                    piece[i] = u32x4_t{0, 0, 0, 0};
+                    own_pieces[i * THREADS] = piece[i];
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    largest = __builtin_elementwise_max(largest, __builtin_bit_cast(u16x2_t, piece[i][e] & 0x7fff7fffu));
             }
+            if (largest[0] >= 0x7f80 || largest[1] >= 0x7f80)
+#pragma unroll
+                for (int i = 0; i < PIECES; ++i)
+                    if (holds_infinite(piece[i])) {
+                        const int r = (thread + i * THREADS) / CHUNKS;
+                        atomicOr(&infinite[r / 32], 1u << (r % 32));
+                    }
             __syncthreads();
             rows_infinite = uint64_t(unsigned(uniform(int(infinite[0])))) | uint64_t(unsigned(uniform(int(infinite[1])))) << 32;
         }
@@ -411,7 +452,8 @@ template <int DIM, bool SHARED> __global__ __launch_bounds__(THREADS, DIM == 64 
         }
         if (works) {
             const float reference = top == -INFINITY ? 0.f : top;
-            multiply_keys(next_keys, next_score);
+            if constexpr (AHEAD)
+                multiply_keys(next_keys, next_score);
             bf16x8_t weights[4];
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
@@ -438,55 +480,64 @@ template <int DIM, bool SHARED> __global__ __launch_bounds__(THREADS, DIM == 64 
                         bf16x8_t, i16x8_t{lower[0], lower[1], lower[2], lower[3], upper[0], upper[1], upper[2], upper[3]});
                     acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, weights[u], acc[d], 0, 0, 0);
                 }
+            look_ahead();
             // The order asked of the compiler: every matrix instruction is followed by vector instructions that fill
             // its 32 cycles and by the reads of an operand to come (left alone it put the products of the scores in a
-            // row: 2264 against 2177 us at 2048 tokens after 30001, heads of 128). Heads of 64 have half the matrix
-            // instructions for as many of the others: 10 and 4 of them after each took 161 us where 5 and 2 took 169.
-            constexpr int AFTER_SCORES = DIM == 64 ? 10 : 5, AFTER_VALUES = DIM == 64 ? 4 : 2;
-            __builtin_amdgcn_sched_group_barrier(DS_READS, 4, 0);
+            // row: 2264 against 2177 us at 2048 tokens after 30001).
+            if constexpr (AHEAD) {
+                __builtin_amdgcn_sched_group_barrier(DS_READS, 4, 0);
 #pragma unroll
-            for (int i = 0; i < 2 * DIM / 16; ++i) {
-                __builtin_amdgcn_sched_group_barrier(MATRIX, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(DS_READS, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(VECTOR, AFTER_SCORES, 0);
-            }
+                for (int i = 0; i < 2 * DIM / 16; ++i) {
+                    __builtin_amdgcn_sched_group_barrier(MATRIX, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(DS_READS, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(VECTOR, 5, 0);
+                }
 #pragma unroll
-            for (int i = 0; i < TILE / 16 * DIM / 32; ++i) {
-                __builtin_amdgcn_sched_group_barrier(MATRIX, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(DS_READS, 2, 0);
-                __builtin_amdgcn_sched_group_barrier(VECTOR, AFTER_VALUES, 0);
+                for (int i = 0; i < TILE / 16 * DIM / 32; ++i) {
+                    __builtin_amdgcn_sched_group_barrier(MATRIX, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(DS_READS, 2, 0);
+                    __builtin_amdgcn_sched_group_barrier(VECTOR, 2, 0);
+                }
             }
+        } else {
+            look_ahead();
         }
-        wanted = next_wanted;
         asm volatile("" ::: "memory");
         pipeline_barrier<0>();
         asm volatile("" ::: "memory");
     };
 
     if (first < end) {
-        page = page_at(first);
-        wanted = wanted_rows(first, page);
-        at = place(first, page);
-        fetch(p.cache.k, key_from, at, first, page, keys0);
-        fetch(p.cache.v, value_from, at, first, page, values0);
-        page = page_at(first + 1);
-        next_page = page_at(first + 2);
-        if (first + 1 < end) {
-            at = place(first + 1, page);
-            fetch(p.cache.k, key_from, at, first + 1, page, keys1);
-        }
+        const int raw0 = load_page(first), raw1 = load_page(first + 1), raw2 = load_page(first + 2);
+        raw3 = load_page(first + 3);
+        const int page0 = checked(first, raw0);
+        page1 = checked(first + 1, raw1);
+        page2 = checked(first + 2, raw2);
+        asm volatile("" : "+v"(page1), "+v"(page2), "+v"(raw3));
+        const int64_t at0 = place(first, page0);
+        at1 = place(first + 1, page1);
+        fetch(p.cache.k, key_from, at0, first, page0, keys0);
+        fetch(p.cache.v, value_from, at0, first, page0, values0);
+        if (AHEAD && first + 1 < end)
+            fetch(p.cache.k, key_from, at1, first + 1, page1, keys1);
+        at2 = place(first + 2, page2);
+        wanted = wanted_rows(first, page0);
+        wanted1 = wanted_rows(first + 1, page1);
+        wanted2 = wanted_rows(first + 2, page2);
         pipeline_barrier<0>();
         asm volatile("" ::: "memory");
         f32x16_t even[2], odd[2];
-        multiply_keys(keys0, even);
-        asm volatile("" ::: "memory");
-        pipeline_barrier<0>();
+        if constexpr (AHEAD) {
+            multiply_keys(keys0, even);
+            asm volatile("" ::: "memory");
+            pipeline_barrier<0>();
+        }
         asm volatile("" ::: "memory");
         for (int tile = first; tile < end; tile += 2) {
-            turn(tile, even, odd, keys0, keys1, values0, values1);
+            turn(tile, even, AHEAD ? odd : even, keys0, keys1, values0, values1);
             if (tile + 1 >= end)
                 break;
-            turn(tile + 1, odd, even, keys1, keys0, values1, values0);
+            turn(tile + 1, AHEAD ? odd : even, even, keys1, keys0, values1, values0);
         }
     }
 
