@@ -158,35 +158,36 @@ struct Block {
     int row0, rows;                        // the block's first row, how many rows the sequence has from there on
 };
 
-// The block of a number (first_block); false for one that is not used. The lengths travel with the starts: a
-// small call is a chain of trips to memory.
+// The block of a number (first_block); false for one that is not used. A sequence's first block number grows with
+// the sequence, so every wavefront looks for it among 64 at a time, without meeting the others; what is known of
+// the sequence travels with the starts: a small call is a chain of trips to memory
+// (one sequence a thread and the finder's words through LDS: 12 tokens past 165 8.6 / 8.3 us).
 __device__ __forceinline__ bool find_block(const PrefillParams &p, int number, Block &block)
 {
-    __shared__ int found[4];
     // the last blocks of a causal sequence see most: they start first
     block.kv_head = number % p.cache.kv_heads;
-    const int wanted = p.row_blocks - 1 - number / p.cache.kv_heads;
-    if (threadIdx.x == 0)
-        found[0] = -1;
-    __syncthreads();
-    for (int b = threadIdx.x; b < p.batch; b += THREADS) {
-        const int begin = first_token(p, b), end = first_token(p, b + 1), length = live_positions(p.table, p.cache, b);
-        if (first_block(begin, p.group, ROWS, b) <= wanted && wanted < first_block(end, p.group, ROWS, b + 1)) {
-            found[0] = b;
-            found[1] = begin;
-            found[2] = end - begin;
-            found[3] = length;
-        }
+    const int wanted = p.row_blocks - 1 - number / p.cache.kv_heads, lane = threadIdx.x % 64;
+    int low = 0, count = p.batch;
+    for (;;) {
+        const int step = (count + 63) / 64, sequence = low + min(lane * step, count - 1);
+        const int begin = first_token(p, sequence), end = first_token(p, sequence + 1);
+        const int length = live_positions(p.table, p.cache, sequence);
+        const uint64_t before = __ballot(lane * step < count && first_block(begin, p.group, ROWS, sequence) <= wanted);
+        if (before == 0)
+            return false;
+        const int last = 63 - __builtin_clzll(before);
+        low += last * step;
+        count = min(step, count - last * step);
+        if (step > 1)
+            continue;
+        block.sequence = low;
+        block.token0 = __builtin_amdgcn_readlane(begin, last);
+        block.tokens = __builtin_amdgcn_readlane(end, last) - block.token0;
+        block.length = __builtin_amdgcn_readlane(length, last);
+        block.row0 = (wanted - first_block(block.token0, p.group, ROWS, low)) * ROWS;
+        block.rows = block.tokens * p.group - block.row0;
+        return block.row0 >= 0 && block.rows > 0;
     }
-    __syncthreads();
-    block.sequence = uniform(found[0]);
-    block.token0 = uniform(found[1]);
-    // (starts that do not ascend may give a number to several sequences, and a mixture of them: it stays in bounds)
-    block.tokens = min(uniform(found[2]), p.tokens - block.token0);
-    block.length = uniform(found[3]);
-    block.row0 = (wanted - first_block(block.token0, p.group, ROWS, block.sequence)) * ROWS;
-    block.rows = block.tokens * p.group - block.row0;
-    return block.sequence >= 0 && block.row0 >= 0 && block.rows > 0;
 }
 
 // SHARED: blockIdx.y of `shares` workgroups takes its part of the tiles and leaves what it has for the join.
@@ -639,7 +640,7 @@ int64_t prefill_blocks(int batch, int tokens, int group) { return int64_t(tokens
 
 // Over how many workgroups the positions of a block of rows are divided: as many as fill the chip where the
 // blocks alone do not, with a few tiles each. Measured, one workgroup / shares: 7 sequences of up to 41 tokens past
-// 2000 positions 56 / 28 us; 15 of one token past 7000 154 / 27; 64 tokens past 16000 389 / 57.
+// 2000 positions 56 / 27 us; 15 of one token past 7000 154 / 20; 64 tokens past 16000 389 / 57.
 int prefill_shares(int64_t blocks, int dim, int64_t positions, int compute_units)
 {
     const int64_t room = int64_t(dim == 64 ? 3 : 2) * compute_units / (blocks > 0 ? blocks : 1);

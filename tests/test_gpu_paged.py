@@ -422,6 +422,20 @@ def test_few_rows_over_a_long_past_with_values_that_are_not_numbers(dim, device)
     assert reference.within(got, want, allowed)
 
 
+@pytest.mark.parametrize("batch, every", [(65, 1), (300, 3), (4200, 60)])
+def test_prefill_finds_its_rows_among_many_sequences(batch, every, device):
+    # most sequences have no new tokens
+    new = [(b // every) % 3 + 1 if b % every == every - 1 else 0 for b in range(batch)]
+    lengths = [n + b % 7 for b, n in enumerate(new)]
+    k, v, table = reference.paged_case(2575, lengths, page_size=16, kv_heads=1, dim=64, device=device)
+    q = queries(2576, sum(new), 50, 64, device)
+    held = torch.tensor(lengths, dtype=torch.int32, device=device)
+    got = _kernels.paged_prefill_attention(q, k, v, table, held, starts_of(new, device))
+    some = [b for b in range(batch) if new[b]]
+    want, allowed = reference.attention_rows(q, k, v, table[some], [lengths[b] for b in some], [new[b] for b in some])
+    assert reference.within(got, want, allowed)
+
+
 def test_starts_in_no_order_stay_inside(device):
     batch, tokens = 600, 70
     k, v, table = reference.paged_case(2570, [30] * batch, page_size=16, kv_heads=2, dim=64, device=device)
