@@ -571,9 +571,15 @@ hipError_t launch_paged_decode(hipStream_t stream, int batch, int q_heads, int d
     const bool large = cache.page_shift >= 4 && cache.slot_stride < (int64_t(1) << 26);
     if (shares == 0) {
         const dim3 grid(items, batch);
-        // (with less than a workgroup per compute unit eight wavefronts each: 8 items of 129 positions 8.0 / 7.3 us)
-        if (int64_t(batch) * items < compute_units)
+        // With less than a workgroup per compute unit eight wavefronts each (8 items of 129 positions, four / eight: 8.0 /
+        // 7.3 us); with more workgroups than two per compute unit, as many as fit of four wavefronts, and few positions
+        // two each (four / two: 1024 items of 64 positions 11.8 / 9.3 us, of 256 25.9 / 25.1, of 512 46.0 / 46.1; 512 of
+        // 64 6.9 / 6.9).
+        const int64_t workgroups = int64_t(batch) * items;
+        if (workgroups < compute_units)
             launch_whole<8>(stream, dim, large, grid, p);
+        else if (workgroups > 2 * compute_units && decode_positions(capacity, see) <= 256)
+            launch_whole<2>(stream, dim, large, grid, p);
         else
             launch_whole<4>(stream, dim, large, grid, p);
         return launch_status();

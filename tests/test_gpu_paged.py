@@ -61,6 +61,15 @@ def test_decode_divided_over_workgroups(device, lengths):
     check_decode(device, 300, lengths, q_heads=8, kv_heads=2, dim=128, page_size=16)
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("page_size", [4, 16])
+@pytest.mark.parametrize("longest,window", [(1, 0), (67, 0), (256, 0), (600, 90)])
+def test_decode_many_sequences_of_few_positions(device, dim, page_size, longest, window):
+    # several workgroups per compute unit
+    lengths = [b * 41 % (longest + 1) for b in range(70)]
+    check_decode(device, 350, lengths, q_heads=8, kv_heads=8, dim=dim, page_size=page_size, window=window, sinks=3)
+
+
 @pytest.mark.parametrize("layout", ["together", "heads first"])
 def test_decode_layouts_of_the_cache(device, layout):
     check_decode(device, 400, [5, 200, 1030], q_heads=9, kv_heads=3, dim=64, page_size=16, layout=layout)
