@@ -19,11 +19,11 @@
 // refer to is moved only when a score exceeds it by 2^8; weights are rounded to BF16 for the second product,
 // their sum is kept in FP32.
 //
-// Measured, 64 query and 8 key-value heads of 128: 2048 tokens after 30001 positions 1.97 ms, 1055 TFLOP/s; 4096 tokens
-// from the beginning 288 us, 955 TFLOP/s (a large matrix product reaches 1410). Heads of 128 are bound by the power
-// that the matrix units may draw: those are busy 55 % of the cycles, at 1.8 GHz. Six prompts of 28 query and 4 key-value
-// heads of 64 behind a window of 1024: 156 us, 645 TFLOP/s; the work on scores is the same for half the products (matrix
-// units busy 35 %, vector instructions issued in 67 % of the cycles); fetching tiles is 16 us of it, masks 12.
+// Measured, 64 query and 8 key-value heads of 128: 2048 tokens after 30001 positions 1.90 ms, 1096 TFLOP/s; 4096 tokens
+// from the beginning 272 us, 1010 TFLOP/s (a large matrix product reaches 1410). Heads of 128 are bound by the power
+// that the matrix units may draw: those are busy 62 % of the cycles, at 1.7 to 1.8 GHz. Six prompts of 28 query and 4
+// key-value heads of 64 behind a window of 1024: 152 us, 665 TFLOP/s; the work on scores is the same for half the
+// products (matrix units busy 36 %, vector instructions issued in 72 % of the cycles).
 #include "common.hpp"
 #include "device.hpp"
 #include "dma.hpp"
