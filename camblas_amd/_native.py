@@ -101,6 +101,7 @@ SIGNATURES = {
     "add_residual_squares": ([_P, _I, _I, _P, _P, _P, _P], _I),
     "fp8_moe_decode": ([_P, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _F, _P], _I),
     "qk_norm_rope_append": ([_P, _I, _I, _I, _F, _I, _F, _P, _P, _P, _P, _P, _L, _P, _L, _P], _I),
+    "qk_norm_rope_append_wide_theta": ([_P, _I, _I, _I, _D, _I, _F, _P, _P, _P, _P, _P, _L, _P, _L, _P], _I),
     "paged_decode_workspace_size": ([_P, _I, _I, _P, _I, _I, _I], _SZ),
     "paged_decode_attention": ([_P, _I, _I, _P, _P, _L, _I, _P, _I, _I, _F, _P, _L, _P, _SZ, _P, _L], _I),
     "paged_prefill_workspace_size": ([_P, _I, _I, _I, _P, _I, _I, _I], _SZ),

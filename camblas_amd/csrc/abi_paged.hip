@@ -3,6 +3,7 @@
 #include "entry.hpp"
 #include "paged_cache.hpp"
 
+#include <cfloat>
 #include <cmath>
 #include <cstdint>
 
@@ -96,6 +97,18 @@ extern "C" int camblas_cuda_qk_norm_rope_append(camblas_cuda_context *context, i
                                                 const void *qkv, int64_t token_stride, void *queries,
                                                 int64_t queries_stride, const camblas_cuda_paged_cache *cache)
 {
+    return camblas_cuda_qk_norm_rope_append_wide_theta(context, tokens, q_heads, rotary_dim, theta, weight_dtype, epsilon,
+                                                       q_weight, k_weight, positions, slots, qkv, token_stride, queries,
+                                                       queries_stride, cache);
+}
+
+extern "C" int camblas_cuda_qk_norm_rope_append_wide_theta(camblas_cuda_context *context, int tokens, int q_heads,
+                                                           int rotary_dim, double theta, int weight_dtype, float epsilon,
+                                                           const void *q_weight, const void *k_weight,
+                                                           const int32_t *positions, const int64_t *slots, const void *qkv,
+                                                           int64_t token_stride, void *queries, int64_t queries_stride,
+                                                           const camblas_cuda_paged_cache *cache)
+{
     Entry entry(context);
     return entry.run([&] {
         if (!valid_cache(cache))
@@ -103,7 +116,7 @@ extern "C" int camblas_cuda_qk_norm_rope_append(camblas_cuda_context *context, i
         const int64_t width = (int64_t(q_heads) + 2 * int64_t(cache->kv_heads)) * cache->dim;
         const bool shaped = q_heads >= 1 && q_heads <= 65536 &&
                             within({{tokens, 0, 1 << 25, 1}, {rotary_dim, 0, cache->dim, 16}}) &&
-                            std::isfinite(theta) && theta > 0 && storage_in(weight_dtype, {0, 2}) && std::isfinite(epsilon) && epsilon >= 0 &&
+                            theta >= 0x1p-149 && theta <= FLT_MAX && storage_in(weight_dtype, {0, 2}) && std::isfinite(epsilon) && epsilon >= 0 &&
                             within({{token_stride, 0, FAR, 8}, {queries_stride, 0, FAR, 8}}) &&
                             (tokens <= 1 || queries_stride >= int64_t(q_heads) * cache->dim);
         if (!shaped)

@@ -94,8 +94,8 @@ Tensor append(const Tensor &qkv, const Tensor &positions, const Tensor &slots, c
     Tensor queries = output_rows(out, tokens, q_heads, dim, qkv);
     const int64_t queries_stride = row_stride("out", queries, tokens, q_heads, dim, device);
     camblas_cuda_context *context = context_for(device.index(), current_default_algorithm());
-    succeed(camblas_cuda_qk_norm_rope_append(
-                context, int(tokens), int(q_heads), rotary_dim ? as_int("rotary_dim", *rotary_dim) : int(dim), float(theta),
+    succeed(camblas_cuda_qk_norm_rope_append_wide_theta(
+                context, int(tokens), int(q_heads), rotary_dim ? as_int("rotary_dim", *rotary_dim) : int(dim), theta,
                 q_weight ? storage_code(*q_weight) : 0, float(epsilon), q_weight ? q_weight->const_data_ptr() : nullptr,
                 k_weight ? k_weight->const_data_ptr() : nullptr, positions.const_data_ptr<int32_t>(),
                 slots.const_data_ptr<int64_t>(), qkv.const_data_ptr(), stride, queries.mutable_data_ptr(), queries_stride,

@@ -6,9 +6,9 @@
 //   (lo, hi) -> (lo cos a - hi sin a, hi cos a + lo sin a)   lo = y[i], hi = y[i + rotary / 2],
 //                                                        a = position * theta^(-2 i / rotary)
 //
-// All of it in FP32 with one rounding to BF16 at the end. The angle is formed in FP64 as a number of
-// turns, of which the whole ones are dropped before the FP32 sine and cosine: at position 2^20 an angle
-// in FP32 is off by up to 2^-4 of a radian.
+// All of it in FP32 with one rounding to BF16 at the end. The angle is formed in FP64, from a base in FP64, as a
+// number of turns, of which the whole ones are dropped before the FP32 sine and cosine: at position 2^20 an angle
+// in FP32 is off by up to 2^-4 of a radian, and one whose base is rounded to FP32 by up to 2^-8.
 //
 // A lane owns eight pairs of a head: dims 8 j .. 8 j + 7 and rotary / 2 further (dims that are not
 // rotated are dealt in the same way: two runs of eight), so dim / 16 lanes hold a head, the sum of squares
@@ -101,7 +101,9 @@ template <int DIM> __global__ __launch_bounds__(APPEND_WAVES * 64) void qk_norm_
     const int wave = threadIdx.x / 64;
     {
         // theta^(-2 lane / rotary) as a product over the bits of the lane (64 values worked out on the host were 2 of
-        // the 6 us of a small call); twelve roundings of 2^-53 are lost in that of the turn
+        // the 6 us of a small call). A square doubles the relative error of its power and rounds once, so that lane i is
+        // off by (3 i + 8) 2^-53 of its turn at most; turns get shorter faster than that grows: under 2^-18 of a radian
+        // at position 2^31 and a base of 10^4 or more.
         double turn = double(p.positions[token]) * (1 / 6.283185307179586476925);
 #pragma unroll
         for (int bit = 0; bit < 6; ++bit)
@@ -196,7 +198,7 @@ template <int DIM> __global__ __launch_bounds__(APPEND_WAVES * 64) void qk_norm_
 }
 } // namespace
 
-hipError_t launch_qk_norm_rope_append(hipStream_t stream, int tokens, int q_heads, int dim, int rotary, float theta,
+hipError_t launch_qk_norm_rope_append(hipStream_t stream, int tokens, int q_heads, int dim, int rotary, double theta,
                                       float epsilon, const void *q_weight, const void *k_weight, bool weight_bf16,
                                       const int32_t *positions, const int64_t *slots, const void *qkv,
                                       int64_t token_stride, void *q_out, int64_t out_stride, const PagedCache &cache)
@@ -216,7 +218,7 @@ hipError_t launch_qk_norm_rope_append(hipStream_t stream, int tokens, int q_head
     p.token_stride = token_stride;
     p.out_stride = out_stride;
     p.cache = cache;
-    double power = rotary ? std::pow(double(theta), -2.0 / rotary) : 1;
+    double power = rotary ? std::pow(theta, -2.0 / rotary) : 1;
     for (double &of : p.powers) {
         of = power;
         power *= power;

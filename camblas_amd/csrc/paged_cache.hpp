@@ -13,7 +13,7 @@
 namespace camblas_hip
 {
 // ---- launchers (each returns a hipError_t); what they ask of their arguments is checked by the entry points
-hipError_t launch_qk_norm_rope_append(hipStream_t stream, int tokens, int q_heads, int dim, int rotary, float theta,
+hipError_t launch_qk_norm_rope_append(hipStream_t stream, int tokens, int q_heads, int dim, int rotary, double theta,
                                       float epsilon, const void *q_weight, const void *k_weight, bool weight_bf16,
                                       const int32_t *positions, const int64_t *slots, const void *qkv,
                                       int64_t token_stride, void *q_out, int64_t out_stride, const PagedCache &cache);

@@ -421,6 +421,13 @@ int camblas_cuda_qk_norm_rope_append(camblas_cuda_context *context, int tokens, 
                                      const void *k_weight, const int32_t *positions, const int64_t *slots,
                                      const void *qkv, int64_t token_stride, void *queries, int64_t queries_stride,
                                      const camblas_cuda_paged_cache *cache);
+/* The same for a base that FP32 does not hold (a rescaled one: rounded to FP32 it moves an angle by up to
+ * 2^-8 of a radian at position 2^20); theta within FP32's range. */
+int camblas_cuda_qk_norm_rope_append_wide_theta(camblas_cuda_context *context, int tokens, int q_heads, int rotary_dim,
+                                                double theta, int weight_dtype, float epsilon, const void *q_weight,
+                                                const void *k_weight, const int32_t *positions, const int64_t *slots,
+                                                const void *qkv, int64_t token_stride, void *queries,
+                                                int64_t queries_stride, const camblas_cuda_paged_cache *cache);
 /* One new token per sequence: q rows [batch] of q_heads * dim (a multiple of kv_heads heads), at position
  * lengths[b] - 1, over its sequence's positions: all of them (window 0), or the last `window` and the first
  * `sinks`. output = softmax(scale q k^T) v per head, scale positive; FP32 sums, weights rounded to BF16 for the

@@ -167,3 +167,10 @@ def test_the_reference_agrees_with_a_dense_softmax():
     # a rounding of the output alone is allowed, one of twice that size is not
     assert reference.within(got.to(torch.bfloat16), got, allowed)
     assert not reference.within(got + 3 * allowed, got, allowed)
+
+
+def test_the_append_with_a_wide_base_refuses_a_missing_context():
+    lib = _native.library()
+    described = ct.byref(_native.PagedCache())
+    assert lib.camblas_cuda_qk_norm_rope_append_wide_theta(None, 1, 1, 64, 1e4, 0, 1e-6, None, None, None, None, None, 64, None, 64, described) == -1
+    assert b"missing context" in lib.camblas_cuda_error(None)

@@ -264,6 +264,34 @@ def test_append(device, tokens, q_heads, kv_heads, dim, rotary, norm, page_size)
         assert torch.equal(cache.view(-1, kv_heads, dim)[others], old.view(-1, kv_heads, dim)[others])
 
 
+@pytest.mark.parametrize("theta", [500000 * 8 ** (128 / 126), 10000 * 4 ** (128 / 126)])
+@pytest.mark.parametrize("dim,rotary", [(64, 64), (128, 64), (128, 128)])
+def test_append_bases_that_32_bits_do_not_hold(device, theta, dim, rotary):
+    """Rescaled bases, up to the farthest position. Allowed is 2^-17 of a pair: a turn of lane i is a product of i powers
+    of one (relative error (3 i + 8) 2^-53 at most: one step for the power, doubled and rounded with every square, six
+    products, two roundings of the position's turn) and theta^(-2 i / rotary) 2^31 / 2 pi turns long, so off by at most 10.5 * 2^-53
+    * 2^28.35 turns = 2^-18.6 radians for the bases and dims here (the largest (3 i + 8) theta^(-2 i / rotary) is 10.5);
+    the reference's angle by 2^-21, the FP32 fraction of a turn, sine, cosine and products by 2^-21 together. These
+    bases rounded to 32 bits are off by up to 2^-10 of a radian at 2^20."""
+    tokens, q_heads, kv_heads = 40, 3, 2
+    assert ct.c_float(theta).value != theta
+    qkv = queries(2150, tokens, q_heads + 2 * kv_heads, dim, device)
+    g = torch.Generator().manual_seed(2151)
+    positions = torch.randint(0, 2**31 - 1, (tokens,), generator=g, dtype=torch.int64).to(torch.int32)
+    positions[:5] = torch.tensor([0, 1, 2**20, 2**30, 2**31 - 1])
+    positions[5:20] = positions[5:20] % 2**20
+    k, v = (torch.zeros(tokens, 1, kv_heads, dim, dtype=torch.bfloat16, device=device) for _ in range(2))
+    got = _kernels.qk_norm_rope_append(qkv, positions.to(device), torch.arange(tokens, device=device), k, v, q_heads=q_heads, kv_heads=kv_heads,
+                                       theta=theta, rotary_dim=rotary)
+    q_want, k_want, q_off, k_off = reference.append(qkv, positions, q_heads=q_heads, kv_heads=kv_heads, q_weight=None, k_weight=None,
+                                                    epsilon=0.0, theta=theta, rotary=rotary)
+    assert reference.within(got, q_want, q_off)
+    assert reference.within(k[:, 0], k_want, k_off)
+    for other in (1e300, 1e-60, math.inf):  # outside of what 32 bits hold at all
+        refused(_kernels.qk_norm_rope_append, qkv, positions.to(device), torch.arange(tokens, device=device), k, v, q_heads=q_heads,
+                kv_heads=kv_heads, theta=other, rotary_dim=rotary)
+
+
 def test_append_in_place_and_into_views_of_one_cache(device):
     tokens, q_heads, kv_heads, dim = 50, 12, 3, 128
     qkv = queries(2100, tokens, q_heads + 2 * kv_heads, dim, device)
