@@ -10,6 +10,9 @@
 #include "device.hpp"
 #include "paged_span.hpp"
 
+#include <cfloat>
+#include <cmath>
+
 namespace camblas_hip
 {
 // ---- launchers (each returns a hipError_t); what they ask of their arguments is checked by the entry points
@@ -35,5 +38,13 @@ __device__ __forceinline__ unsigned round_pair(float lo, float hi)
     typedef float pair_f32 __attribute__((ext_vector_type(2)));
     typedef __bf16 pair_bf16 __attribute__((ext_vector_type(2)));
     return __builtin_bit_cast(unsigned, __builtin_convertvector((pair_f32{lo, hi}), pair_bf16));
+}
+
+// What the weighted sum of a head is multiplied by at the end, from the running maximum and the sum of weights. A head
+// that has seen no position keeps a maximum of minus infinity and gives zeros. One whose scores were all minus
+// infinity has a finite maximum (no score is below it) and a sum of zero: 0 / 0, NaN. A sum that is NaN stays NaN.
+__device__ __forceinline__ float normaliser(float top, float sum)
+{
+    return sum != 0.f ? 1.f / sum : top == -INFINITY ? 0.f : __builtin_nanf("");
 }
 } // namespace camblas_hip

@@ -241,6 +241,7 @@ __device__ __forceinline__ void work_item(const DecodeParams &p, const unsigned 
         run.acc[w] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 
     const int end = min(last * WAVES, span.tiles);
+    unsigned met = 0; // whether a position was seen at all
     __syncthreads(); // (outputs of the item before may still be read)
     int tile = __builtin_amdgcn_readfirstlane(first * WAVES + wave);
     if (tile < end) {
@@ -259,6 +260,7 @@ __device__ __forceinline__ void work_item(const DecodeParams &p, const unsigned 
             park_keys<DIM>(k, lane, keys);
             if (tile < end)
                 load_rows<DIM, LARGE>(p, p.cache.k, base, page, head_at, lane, along, k);
+            met |= mask;
             const bf16x8_t weights = weigh<DIM>(scale, mask, q, lane, keys, run);
             add_values<DIM>(mask, weights, v, lane, run);
             if (tile >= end)
@@ -269,6 +271,8 @@ __device__ __forceinline__ void work_item(const DecodeParams &p, const unsigned 
             page = fetch_page(p, row, base, lane);
         }
     }
+    if (met && run.top == -INFINITY) // (scores of minus infinity only)
+        run.top = -FLT_MAX;
     run.total += __shfl_xor(run.total, 16);
     run.total += __shfl_xor(run.total, 32);
     __syncthreads(); // (keys of other wavefronts may still be read)
@@ -300,8 +304,7 @@ __device__ __forceinline__ void work_item(const DecodeParams &p, const unsigned 
             denominator = fmaf(factor, wave_l[w][h], denominator);
         }
         if (slot < 0) {
-            // (no position seen: zero; a sum that is NaN stays NaN)
-            numerator *= denominator == 0.f ? 0.f : 1.f / denominator;
+            numerator *= normaliser(best, denominator);
             *reinterpret_cast<u32x2_t *>(p.out + int64_t(item.sequence) * p.out_stride + int64_t(item.head0 + h) * DIM + d) =
                 u32x2_t{round_pair(numerator[0], numerator[1]), round_pair(numerator[2], numerator[3])};
         } else {
@@ -506,7 +509,7 @@ template <int DIM> __global__ __launch_bounds__(JOIN_THREADS) void paged_decode_
 #pragma unroll
         for (int w = 0; w < JOIN_WAVES; ++w)
             denominator += wave_sums[w];
-        out[thread] = float_to_bf16_bits(denominator == 0.f ? 0.f : numerator / denominator);
+        out[thread] = float_to_bf16_bits(denominator != 0.f ? numerator / denominator : numerator * normaliser(top, denominator));
     }
 }
 } // namespace

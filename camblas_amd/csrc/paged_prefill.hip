@@ -44,6 +44,7 @@ struct PrefillParams {
     Visibility see;
     const int32_t *starts; // [batch + 1]: first token of each sequence
     float scale;           // times log2(e)
+    float lowest;          // no finite score is below it, and its product with the scale is finite
     const unsigned short *q;
     unsigned short *out;
     int64_t q_stride, out_stride;
@@ -360,8 +361,10 @@ template <int DIM, bool SHARED> __global__ __launch_bounds__(THREADS, DIM == 64 
         const bool whole = wanted == ~uint64_t(0) && base + TILE - 1 <= first_query &&
                            (p.see.window <= 0 || base > last_query - p.see.window || base + TILE <= p.see.sinks);
         uint64_t rows_infinite = 0;
+        float highest = p.lowest; // a row that sees a position has a finite maximum, whatever its scores are
         if (!whole) { // (the same in every wavefront)
             const uint64_t own = seen_rows(base) >> (4 * half);
+            highest = own ? p.lowest : -INFINITY;
             if (works)
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
@@ -402,7 +405,6 @@ template <int DIM, bool SHARED> __global__ __launch_bounds__(THREADS, DIM == 64 
             rows_infinite = uint64_t(unsigned(uniform(int(infinite[0])))) | uint64_t(unsigned(uniform(int(infinite[1])))) << 32;
         }
         if (works) {
-            float highest = -INFINITY;
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -563,8 +565,7 @@ template <int DIM, bool SHARED> __global__ __launch_bounds__(THREADS, DIM == 64 
                 *reinterpret_cast<f32x4_t *>(to + 32 * d + 8 * g) =
                     f32x4_t{acc[d][4 * g], acc[d][4 * g + 1], acc[d][4 * g + 2], acc[d][4 * g + 3]};
     } else {
-        // (no position seen: zero; a sum that is NaN stays NaN)
-        const float inverse = sum == 0.f ? 0.f : 1.f / sum;
+        const float inverse = normaliser(top, sum);
         // The two lanes of a row hold four dims each of every eight: the upper gives its half of the even eights for
         // the lower's half of the odd ones, and each writes eight dims in one piece.
         unsigned short *to = p.out + int64_t(token) * p.out_stride + int64_t(head) * DIM + 8 * half;
@@ -631,7 +632,7 @@ template <int DIM> __global__ __launch_bounds__(THREADS) void paged_prefill_join
     }
     if (head >= q_heads)
         return;
-    o *= sum == 0.f ? 0.f : 1.f / sum;
+    o *= normaliser(top, sum);
     *reinterpret_cast<u32x2_t *>(p.out + int64_t(token) * p.out_stride + int64_t(head) * DIM + d) =
         u32x2_t{round_pair(o[0], o[1]), round_pair(o[2], o[3])};
 }
@@ -686,6 +687,7 @@ hipError_t launch_paged_prefill(hipStream_t stream, int batch, int tokens, int q
     p.see = see;
     p.starts = starts;
     p.scale = scale * LOG2E;
+    p.lowest = -FLT_MAX / (p.scale > 1.f ? 2.f * p.scale : 1.f);
     p.q = static_cast<const unsigned short *>(q);
     p.out = static_cast<unsigned short *>(out);
     p.q_stride = q_stride;

@@ -431,7 +431,8 @@ int camblas_cuda_qk_norm_rope_append_wide_theta(camblas_cuda_context *context, i
 /* One new token per sequence: q rows [batch] of q_heads * dim (a multiple of kv_heads heads), at position
  * lengths[b] - 1, over its sequence's positions: all of them (window 0), or the last `window` and the first
  * `sinks`. output = softmax(scale q k^T) v per head, scale positive; FP32 sums, weights rounded to BF16 for the
- * second product, one rounding at the end; zeros where a token sees nothing. The cache's rows that a token does
+ * second product, one rounding at the end; zeros where a token sees nothing (NaN where it sees positions whose scores are
+ * all minus infinity: a softmax of 0 / 0). The cache's rows that a token does
  * not see do not reach its output, whatever they hold. workspace: ..._workspace_size() bytes (0: none), 16-byte
  * aligned, written before it is read; calls that may run at the same time need one each. No atomics: results repeat bit for
  * bit on one device. */

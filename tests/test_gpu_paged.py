@@ -214,6 +214,38 @@ def test_prefill_infinite_and_nan_values_reach_only_who_sees_them(device, dim, p
     assert torch.isnan(want).any() and torch.isinf(want).any()
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("past,window,scale", [(0, 0, None), (3000, 0, None), (3000, 40, None), (3000, 1500, None), (0, 0, 5.0), (3000, 0, 5.0)])
+def test_scores_of_minus_infinity(device, dim, past, window, scale):
+    """Keys of minus infinity take a weight of zero; where a token sees such keys only, the softmax is 0 / 0 and the output
+    NaN, not the zeros of a token that sees nothing."""
+    new, q_heads, kv_heads, page_size = 70, 6, 2, 16
+    lengths = [past + new, 5, 0, 3]
+    k, v, table = reference.paged_case(760, lengths, page_size=page_size, kv_heads=kv_heads, dim=dim, device=device)
+    hidden = list(range(0, past + 20)) + list(range(past + 50, past + 64))  # of the first sequence, for every head
+    place = torch.tensor(hidden)
+    page = table[0].cpu()[place // page_size].long().to(device)
+    k[page, (place % page_size).to(device), :, 3] = -math.inf
+    k[int(table[1, 0]), :5, 1, 7] = -math.inf  # all of the second's, one head
+    table[3, :] = -1  # no page: nothing is seen
+    q = queries(761, new + 5 + 3, q_heads, dim, device)
+    q[:, :, 3], q[:, :, 7] = q[:, :, 3].abs() + 0.1, q[:, :, 7].abs() + 0.1
+    held = torch.tensor(lengths, dtype=torch.int32, device=device)
+    counts = [new, 5, 0, 3]
+    got = _kernels.paged_prefill_attention(q, k, v, table, held, starts_of(counts, device), window=window, sinks=0, scale=scale)
+    want, allowed = reference.attention_rows(q, k, v, table, lengths, counts, window=window, sinks=0, scale=scale)
+    assert torch.isnan(want[:20]).all() and not torch.isnan(want[20:50]).any() and torch.isnan(want[new:new + 5, 3:]).all()
+    assert reference.within(got, want, allowed) and not got[new + 5:].any()
+    # single tokens, at a length where all of the first sequence's keys are such and at its end
+    for length in (past + 20, past + new):
+        now = [length, 5, 0, 3]
+        held = torch.tensor(now, dtype=torch.int32, device=device)
+        got = _kernels.paged_decode_attention(q[:4], k, v, table, held, window=window, scale=scale)
+        want, allowed = reference.attention_rows(q[:4], k, v, table, now, [1] * 4, window=window, scale=scale)
+        assert torch.isnan(want[0]).all().item() == (length == past + 20)
+        assert reference.within(got, want, allowed) and not got[2:].any()
+
+
 def test_prefill_one_token_each_equals_decode_within_rounding(device):
     lengths = [1, 70, 1030, 257]
     k, v, table = reference.paged_case(1600, lengths, page_size=16, kv_heads=2, dim=128, device=device)
