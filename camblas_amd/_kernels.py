@@ -804,7 +804,7 @@ def qk_norm_rope_append(qkv, positions, slots, k_cache, v_cache, *, q_heads, kv_
     where keys and values go: page * page_size + place; one outside the cache (-1 for padding rows) writes
     nothing. k_cache and v_cache are BF16 [pages, page_size, kv_heads, dim] of one layout, dim 64 or 128, page_size
     a power of two, strides in multiples of eight with contiguous heads (e.g. views of one [pages, 2, page_size,
-    kv_heads, dim] tensor). `out` may be qkv[:, :q_heads].
+    kv_heads, dim] tensor); no two rows of them may share memory. `out` may be qkv[:, :q_heads].
     """
     return _tensor_binding().qk_norm_rope_append(
         qkv, positions, slots, k_cache, v_cache, q_heads, kv_heads, q_weight, k_weight, epsilon, theta, rotary_dim, out)

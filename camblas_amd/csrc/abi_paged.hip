@@ -15,8 +15,8 @@ namespace
 {
 constexpr int64_t FAR = int64_t(1) << 32; // no stride of a row reaches as far (2^33 bytes)
 
-// A cache the kernels can address: whole 16-byte pieces of every head, strides that keep heads, slots
-// and pages apart.
+// A cache the kernels can address: whole 16-byte pieces of every head, strides no shorter than a head. Rows may
+// still share memory: see writable_cache.
 bool valid_cache(const camblas_cuda_paged_cache *cache)
 {
     if (!cache || !usable({{cache->k, 16}, {cache->v, 16}}) || cache->k == cache->v)
@@ -29,6 +29,15 @@ bool valid_cache(const camblas_cuda_paged_cache *cache)
            (cache->page_size == 1 || cache->slot_stride >= cache->dim) &&
            (cache->pages == 1 ||
             within({{cache->page_stride, cache->dim, (int64_t(1) << 46) / cache->pages, 1}})); // (last byte: 2^47)
+}
+
+// No two rows of the cache share memory, those of keys and of values among each other: the append's wavefronts write
+// them in no order. (Attention only reads them.)
+bool writable_cache(const camblas_cuda_paged_cache *cache)
+{
+    const int64_t between = int64_t(reinterpret_cast<uintptr_t>(cache->v)) - int64_t(reinterpret_cast<uintptr_t>(cache->k));
+    return places_apart({cache->pages, cache->page_stride}, {cache->page_size, cache->slot_stride},
+                        {cache->kv_heads, cache->head_stride}, cache->dim, between / int64_t(sizeof(unsigned short)));
 }
 
 PagedCache device_cache(const camblas_cuda_paged_cache *cache)
@@ -121,6 +130,8 @@ extern "C" int camblas_cuda_qk_norm_rope_append_wide_theta(camblas_cuda_context 
                             (tokens <= 1 || queries_stride >= int64_t(q_heads) * cache->dim);
         if (!shaped)
             return entry.refuse("invalid paged append arguments");
+        if (!writable_cache(cache))
+            return entry.refuse("paged append into a cache whose rows share memory");
         if (tokens == 0)
             return 0;
         // (the queries may replace their own un-rotated rows, which a workgroup reads before it writes them)

@@ -4,6 +4,7 @@
 #pragma once
 
 #include <cstdint>
+#include <initializer_list>
 
 #if defined(__HIPCC__)
 #define PAGED_INLINE __host__ __device__ __forceinline__
@@ -114,6 +115,61 @@ inline bool rows_apart(const Rows &a, const Rows &b)
     int64_t along = (int64_t(b_begin) - int64_t(a_begin)) % bytes; // of b's rows inside a's
     along += along < 0 ? bytes : 0;
     return along >= a.width * int64_t(sizeof(unsigned short)) && along + b.width * int64_t(sizeof(unsigned short)) <= bytes;
+}
+
+// `count` places `stride` elements apart.
+struct Axis {
+    int64_t count, stride;
+};
+
+// Whether steps along `axes` (fewer than count either way) can bring `offset` within `width` of zero. An axis whose stride
+// is no shorter than what the ones behind it span leaves two steps to try; `tries` bounds the others, and
+// running out of them counts as yes.
+inline bool steps_reach(const Axis *axes, int rank, int64_t offset, int64_t width, int &tries)
+{
+    if (--tries < 0)
+        return true;
+    if (rank == 0)
+        return -width < offset && offset < width;
+    int64_t span = width - 1; // of what is left to step along, and a row
+    for (int i = 1; i < rank; ++i)
+        span += (axes[i].count - 1) * axes[i].stride;
+    const int64_t most = axes[0].count - 1, stride = axes[0].stride;
+    // -span <= offset + step * stride <= span, rounded outwards
+    int64_t step = (-span - offset) / stride - 1, last = (span - offset) / stride + 1;
+    step = step < -most ? -most : step;
+    last = last > most ? most : last;
+    for (; step <= last; ++step)
+        if (steps_reach(axes + 1, rank - 1, offset + step * stride, width, tries))
+            return true;
+    return false;
+}
+
+// Whether all rows of `width` elements along three axes are apart from each other, and from the same rows `offset`
+// elements further (keys and values of a cache). Exact for every layout that slices and transposes of one dense
+// tensor can have; of others a few that take more than 4096 tries are taken to overlap.
+inline bool places_apart(Axis a, Axis b, Axis c, int64_t width, int64_t offset)
+{
+    Axis axes[3];
+    int rank = 0;
+    for (const Axis &axis : {a, b, c}) // in descending order of strides; an axis of one place says nothing
+        if (axis.count > 1) {
+            int at = rank++;
+            for (; at > 0 && axes[at - 1].stride < axis.stride; --at)
+                axes[at] = axes[at - 1];
+            axes[at] = axis;
+        }
+    if (rank > 0 && axes[rank - 1].stride <= 0)
+        return false;
+    int tries = 4096;
+    int64_t span = width - 1; // of the axes behind i, and a row
+    for (int i = rank - 1; i >= 0; --i) { // two rows whose first different step is along axis i
+        for (int64_t step = 1; step < axes[i].count && step * axes[i].stride <= span; ++step)
+            if (steps_reach(axes + i + 1, rank - i - 1, step * axes[i].stride, width, tries))
+                return false;
+        span += (axes[i].count - 1) * axes[i].stride;
+    }
+    return !steps_reach(axes, rank, offset, width, tries);
 }
 
 // `all` steps dealt to `workers` (at most as many) in runs that differ by one step at most: the first step of

@@ -415,7 +415,7 @@ typedef struct camblas_cuda_paged_cache {
  * rounded to BF16 once. The queries go to `queries` (rows of q_heads * dim, queries_stride apart; it may be
  * qkv itself with its stride), keys and values to the slot slots[token] = page * page_size + place of every
  * token. A slot outside the cache writes nothing (padding rows: -1); of two tokens with one slot either may
- * remain, value by value. */
+ * remain, value by value. No two rows of the cache (page, slot, head, keys or values) may share memory. */
 int camblas_cuda_qk_norm_rope_append(camblas_cuda_context *context, int tokens, int q_heads, int rotary_dim,
                                      float theta, int weight_dtype, float epsilon, const void *q_weight,
                                      const void *k_weight, const int32_t *positions, const int64_t *slots,

@@ -121,3 +121,38 @@ def paged_case(seed, lengths, *, page_size, kv_heads, dim, spare=3, device="cuda
         k, v = (t.transpose(1, 2).contiguous().to(device).transpose(1, 2) for t in (k, v))
         return k, v, table.to(device)
     return k.to(device), v.to(device), table.to(device)
+
+
+def cache_layouts():
+    """(keys, values) as views of one tensor, and whether all their rows are apart: [pages, slots, heads, dim]."""
+    def room(*shape):
+        return torch.zeros(*shape, dtype=torch.bfloat16)
+
+    P, S, H, D = 5, 16, 3, 64
+    both = room(2, P, S, H, D)
+    yield both[0], both[1], True
+    both = room(P, 2, S, H, D)
+    yield both[:, 0], both[:, 1], True
+    yield both[:, 1], both[:, 0], True
+    both = room(P, 2, H, S, D)
+    yield both[:, 0].transpose(1, 2), both[:, 1].transpose(1, 2), True
+    both = room(P, S, H, 2 * D)
+    yield both[..., :D], both[..., D:], True
+    yield both[..., :D], both[..., 8:D + 8], False
+    both = room(P, S, 2 * H, D)
+    yield both[:, :, :H], both[:, :, H:], True
+    yield both[:, :, ::2], both[:, :, 1::2], True
+    yield both[:, :, :H], both[:, :, H - 1:-1], False
+    both = room(P, 2 * S, H, D)
+    yield both[:, ::2], both[:, 1::2], True
+    yield both[:, :S], both[:, S:], True
+    yield both[:, :S], both[:, S // 2:S // 2 + S], False
+    both = room(2 * P, S, H, D)
+    yield both[::2], both[1::2], True
+    yield both[:P], both[P:], True
+    yield both[:P], both[P - 1:-1], False
+    yield both[:-1], both[1:], False
+    flat = room(4 * P * S * H * D)
+    yield flat.as_strided((P, S, H, D), (S * D, D, D, 1)), flat.as_strided((P, S, H, D), (S * D, D, D, 1), 2 * P * S * H * D), False
+    yield flat.as_strided((P, S, H, D), (D, P * D, S * P * D, 1)), flat.as_strided((P, S, H, D), (D, P * D, S * P * D, 1), P * S * H * D), True
+    yield flat.as_strided((1, S, 1, D), (0, D, 0, 1)), flat.as_strided((1, S, 1, D), (0, D, 0, 1), S * D), True

@@ -50,3 +50,7 @@ extern "C" int find_apart(int64_t a, int64_t a_count, int64_t a_width, int64_t a
     const auto *memory = reinterpret_cast<const unsigned short *>(uintptr_t(1) << 40);
     return rows_apart(Rows{memory + a, a_count, a_width, a_stride}, Rows{memory + b, b_count, b_width, b_stride});
 }
+extern "C" int find_places_apart(const int64_t *counts, const int64_t *strides, int64_t width, int64_t offset)
+{
+    return places_apart({counts[0], strides[0]}, {counts[1], strides[1]}, {counts[2], strides[2]}, width, offset);
+}

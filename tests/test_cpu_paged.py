@@ -174,3 +174,27 @@ def test_the_append_with_a_wide_base_refuses_a_missing_context():
     described = ct.byref(_native.PagedCache())
     assert lib.camblas_cuda_qk_norm_rope_append_wide_theta(None, 1, 1, 64, 1e4, 0, 1e-6, None, None, None, None, None, 64, None, 64, described) == -1
     assert b"missing context" in lib.camblas_cuda_error(None)
+
+
+def test_caches_whose_rows_share_memory(host):
+    number = ct.c_int64 * 3
+    host.find_places_apart.argtypes = [number, number, ct.c_int64, ct.c_int64]
+    for at, (k, v, apart) in enumerate(reference.cache_layouts()):
+        offset = (v.data_ptr() - k.data_ptr()) // 2
+        assert bool(host.find_places_apart(number(*k.shape[:3]), number(*k.stride()[:3]), k.shape[3], offset)) == apart, at
+    # any strides at all, element by element
+    rng, seen = random.Random(7), set()
+    for _ in range(4000):
+        counts = [rng.choice([1, 1, 2, 3, 4]) for _ in range(3)]
+        width = rng.choice([1, 2, 3])
+        strides = [rng.randint(1, 30) for _ in range(3)]
+        offset = rng.randint(-60, 60)
+        rows = [a * strides[0] + b * strides[1] + c * strides[2] for a in range(counts[0]) for b in range(counts[1]) for c in range(counts[2])]
+        cells = [r + i + o for o in (0, offset) for r in rows for i in range(width)]
+        apart = bool(host.find_places_apart(number(*counts), number(*strides), width, offset))
+        assert apart == (len(set(cells)) == len(cells)), (counts, strides, width, offset)
+        seen.add(apart)
+    assert seen == {True, False}
+    # the largest that an entry lets through: no overflow, and an end
+    for strides in ((2**31 - 8, 2**32, 2**32), (128, 128 * 2**16, 128), (2**16 * 128, 8 * 17, 128)):
+        host.find_places_apart(number(2**15, 2**16, 2**16), number(*strides), 128, 2**46)

@@ -341,6 +341,31 @@ def test_append_in_place_and_into_views_of_one_cache(device):
     assert torch.equal(k2, k) and torch.equal(v2, v)
 
 
+def test_append_into_every_layout_of_a_cache_and_none_that_overlaps(device):
+    tokens, q_heads, kv_heads, dim = 30, 4, 3, 64
+    qkv = queries(2110, tokens, q_heads + 2 * kv_heads, dim, device)
+    positions = torch.arange(tokens, dtype=torch.int32, device=device)
+    slots = torch.arange(tokens, device=device) * 2 + 1
+    options = dict(q_heads=q_heads, kv_heads=kv_heads)
+    want = [torch.zeros(5, 16, kv_heads, dim, dtype=torch.bfloat16, device=device) for _ in range(2)]
+    _kernels.qk_norm_rope_append(qkv, positions, slots, *want, **options)
+    seen = 0
+    for k, v, apart in reference.cache_layouts():
+        if k.shape[2] != kv_heads:
+            continue
+        room = torch.zeros(k.untyped_storage().nbytes() // 2, dtype=torch.bfloat16, device=device)
+        k, v = (room.as_strided(t.shape, t.stride(), t.storage_offset()) for t in (k, v))
+        if apart:
+            _kernels.qk_norm_rope_append(qkv, positions, slots, k, v, **options)
+            assert torch.equal(k[:5], want[0]) and torch.equal(v[:5], want[1])
+        else:
+            with pytest.raises(RuntimeError, match="share memory"):
+                _kernels.qk_norm_rope_append(qkv, positions, slots, k, v, **options)
+            assert not room.any()
+        seen += 1
+    assert seen >= 15
+
+
 def test_a_sequence_from_prompt_to_decode_steps(device):
     """A prompt in two ragged chunks, then single tokens, through append and attention; every attention against
     the definition on what the caches hold."""
