@@ -62,6 +62,13 @@ Tensor output_rows(const std::optional<Tensor> &out, int64_t tokens, int64_t hea
     return out ? *out : at::empty({tokens, heads, dim}, like.options());
 }
 
+// After a call that wrote into `tensor`: a backward that kept it reports that it changed.
+void changed(const Tensor &tensor)
+{
+    if (!tensor.is_inference())
+        torch::autograd::impl::bump_version(tensor);
+}
+
 int as_int(const char *role, int64_t value)
 {
     if (value < 0 || value > INT_MAX)
@@ -101,6 +108,10 @@ Tensor append(const Tensor &qkv, const Tensor &positions, const Tensor &slots, c
                 slots.const_data_ptr<int64_t>(), qkv.const_data_ptr(), stride, queries.mutable_data_ptr(), queries_stride,
                 &cache),
             context);
+    changed(k_cache);
+    changed(v_cache);
+    if (out)
+        changed(queries);
     return queries;
 }
 
@@ -153,6 +164,8 @@ Tensor decode(const Tensor &q, const Tensor &k_cache, const Tensor &v_cache, con
                 lengths.const_data_ptr<int32_t>(), a.window, a.sinks, a.scale, q.const_data_ptr(), a.q_stride,
                 bytes ? workspace.mutable_data_ptr() : nullptr, bytes, a.output.mutable_data_ptr(), a.output_stride),
             context);
+    if (out)
+        changed(a.output);
     return a.output;
 }
 
@@ -175,6 +188,8 @@ Tensor prefill(const Tensor &q, const Tensor &k_cache, const Tensor &v_cache, co
                 a.scale, q.const_data_ptr(), a.q_stride, bytes ? workspace.mutable_data_ptr() : nullptr, bytes,
                 a.output.mutable_data_ptr(), a.output_stride),
             context);
+    if (out)
+        changed(a.output);
     return a.output;
 }
 } // namespace

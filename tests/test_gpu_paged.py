@@ -607,6 +607,44 @@ def test_refusals(device):
     refused(append, qkv, position, slots, k, v, out=torch.empty(2, 7, 128, dtype=torch.bfloat16, device=device), **options)
 
 
+def test_tensors_written_in_place_move_their_version(device):
+    """Another operation's backward must not read what an append or attention has overwritten."""
+    k, v, table = reference.paged_case(2620, [40, 3], page_size=16, kv_heads=2, dim=64, device=device, poison=False)
+    qkv = queries(2621, 2, 8, 64, device)
+    held = torch.tensor([40, 3], dtype=torch.int32, device=device)
+    starts = torch.tensor([0, 1, 2], dtype=torch.int32, device=device)
+    slots = torch.tensor([5, 6], device=device)
+    append, decode, prefill = _kernels.qk_norm_rope_append, _kernels.paged_decode_attention, _kernels.paged_prefill_attention
+    q = append(qkv, held - 1, slots, k, v, q_heads=4, kv_heads=2).clone()
+    calls = {
+        "keys": (k, lambda: append(qkv, held - 1, slots, k, v, q_heads=4, kv_heads=2)),
+        "values": (v, lambda: append(qkv, held - 1, slots, k, v, q_heads=4, kv_heads=2)),
+        "in place": (qkv, lambda: append(qkv, held - 1, slots, k, v, q_heads=4, kv_heads=2, out=qkv[:, :4])),
+        "decode": (torch.zeros_like(q),) * 2, "prefill": (torch.zeros_like(q),) * 2,
+    }
+    calls["decode"] = (calls["decode"][0], lambda: decode(q, k, v, table, held, out=calls["decode"][0]))
+    calls["prefill"] = (calls["prefill"][0], lambda: prefill(q, k, v, table, held, starts, out=calls["prefill"][0]))
+    for name, (written, call) in calls.items():
+        factor = torch.ones_like(written, requires_grad=True)
+        product = factor * written  # keeps `written` for its backward
+        before = written._version
+        with torch.no_grad():
+            call()
+        assert written._version > before, name
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            product.sum().backward()
+    # what is only read, and what a call makes, stays as it was
+    versions = [t._version for t in (q, k, v, table, held)]
+    assert decode(q, k, v, table, held)._version == 0 and prefill(q, k, v, table, held, starts)._version == 0
+    assert versions == [t._version for t in (q, k, v, table, held)]
+    with torch.inference_mode():
+        k2, v2, qkv2, out = k.clone(), v.clone(), qkv.clone(), torch.zeros_like(q)
+        decode(append(qkv2, held - 1, slots, k2, v2, q_heads=4, kv_heads=2), k2, v2, table, held, out=out)
+    # tensors of inference mode have no version; they are written outside of it as before
+    again = decode(append(qkv2, held - 1, slots, k2, v2, q_heads=4, kv_heads=2), k2, v2, table, held, out=out)
+    assert again.data_ptr() == out.data_ptr()
+
+
 def test_the_c_entry_refuses_a_small_or_missing_workspace(device):
     lengths = [2000]
     k, v, table = reference.paged_case(2700, lengths, page_size=16, kv_heads=1, dim=64, device=device)
