@@ -62,6 +62,19 @@ def test_decode_divided_over_workgroups(device, lengths):
 
 
 @pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("page_size", [1, 16])
+@pytest.mark.parametrize("window,sinks", [(1500, 0), (1700, 4), (2500, 64)])
+@pytest.mark.parametrize("lengths", [[3300], [3100, 1, 2600, 700]])
+def test_decode_windows_divided_over_workgroups(device, dim, page_size, window, sinks, lengths):
+    q_heads, kv_heads = 8, 2
+    cache = _native.PagedCache(16, 32, page_size * kv_heads * dim, kv_heads * dim, dim, 4, page_size, kv_heads, dim)  # (sizes only)
+    columns = -(-max(lengths) // page_size) + 2
+    assert _native.library().camblas_cuda_paged_decode_workspace_size(_native.context(device).handle, len(lengths), q_heads, ct.byref(cache), columns,
+                                                                      window, sinks) > 0
+    check_decode(device, 310, lengths, q_heads=q_heads, kv_heads=kv_heads, dim=dim, page_size=page_size, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("page_size", [4, 16])
 @pytest.mark.parametrize("longest,window", [(1, 0), (67, 0), (256, 0), (600, 90)])
 def test_decode_many_sequences_of_few_positions(device, dim, page_size, longest, window):
@@ -167,6 +180,28 @@ def test_prefill_windows_and_first_tokens(device, dim, window, sinks):
     ([130], [1300], 1000, 0)])
 def test_prefill_positions_divided_over_workgroups(device, dim, new, past, window, sinks):
     check_prefill(device, 1250, new, past, q_heads=6, kv_heads=2, dim=dim, page_size=16, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("page_size,window,sinks", [(16, 0, 0), (64, 0, 0), (4, 0, 0), (16, 1200, 70)])
+def test_prefill_long_and_undivided(device, dim, page_size, window, sinks):
+    """Blocks of rows that walk dozens of tiles by themselves; a sample of the tokens against the definition, twice the same."""
+    new, past, q_heads, kv_heads = 2100, 333, 28, 7
+    lengths = [new + past]
+    k, v, table = reference.paged_case(1270, lengths, page_size=page_size, kv_heads=kv_heads, dim=dim, device=device)
+    cache = _native.PagedCache(k.data_ptr(), v.data_ptr(), *k.stride()[:3], *k.shape)
+    assert _native.library().camblas_cuda_paged_prefill_workspace_size(_native.context(device).handle, 1, new, q_heads, ct.byref(cache),
+                                                                       table.shape[1], window, sinks) == 0
+    q = queries(1271, new, q_heads, dim, device)
+    held = torch.tensor(lengths, dtype=torch.int32, device=device)
+    call = lambda: _kernels.paged_prefill_attention(q, k, v, table, held, starts_of([new], device), window=window, sinks=sinks)
+    got = call()
+    assert torch.equal(got, call())
+    g = torch.Generator().manual_seed(1272)
+    for token in [0, 1, 31, 32, new - 1, *torch.randint(0, new, (12,), generator=g).tolist()]:
+        want, allowed = reference.attention_row(q[token].cpu(), k.cpu(), v.cpu(), table[0].cpu(), past + token, window=window, sinks=sinks,
+                                                scale=dim**-0.5)
+        assert reference.within(got[token], want, allowed), token
 
 
 @pytest.mark.parametrize("layout", ["together", "heads first"])
@@ -443,6 +478,24 @@ def test_results_repeat_bit_for_bit_on_two_streams(device):
         for stream in streams:
             with torch.cuda.stream(stream):
                 outs.append(_kernels.paged_decode_attention(q, k, v, table, held))
+    torch.cuda.synchronize()
+    assert all(torch.equal(first, other) for other in outs)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_divided_prefill_repeats_bit_for_bit_on_two_streams(device, dim):
+    new, past = [1, 17, 0, 40], [3001, 0, 77, 2500]
+    lengths = [n + p for n, p in zip(new, past)]
+    k, v, table = reference.paged_case(2410, lengths, page_size=16, kv_heads=2, dim=dim, device=device)
+    q = queries(2411, sum(new), 6, dim, device)
+    held, starts = torch.tensor(lengths, dtype=torch.int32, device=device), starts_of(new, device)
+    first = _kernels.paged_prefill_attention(q, k, v, table, held, starts)
+    torch.cuda.synchronize()
+    streams, outs = [torch.cuda.Stream() for _ in range(2)], []
+    for _ in range(3):
+        for stream in streams:
+            with torch.cuda.stream(stream):
+                outs.append(_kernels.paged_prefill_attention(q, k, v, table, held, starts))
     torch.cuda.synchronize()
     assert all(torch.equal(first, other) for other in outs)
 
