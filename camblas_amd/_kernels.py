@@ -814,7 +814,8 @@ def paged_decode_attention(q, k_cache, v_cache, page_table, lengths, *, scale=No
     """Attention of one new token per sequence, q [batch, q_heads, dim], over pages [pages, page_size,
     kv_heads, dim] found through page_table (int32 [batch, columns]; entries that are no page hold nothing); lengths
     (int32 [batch]) counts the positions of each sequence, the new token's among them. window > 0: only the last
-    `window` positions and the first `sinks` are seen. BF16 [batch, q_heads, dim]; zeros where nothing is seen."""
+    `window` positions and the first `sinks` are seen. BF16 [batch, q_heads, dim]; zeros where nothing is seen. The
+    table's columns decide how the work is divided: one no wider than the sequences need is faster for short ones."""
     return _tensor_binding().paged_decode_attention(q, k_cache, v_cache, page_table, lengths, scale, window, sinks, out)
 
 

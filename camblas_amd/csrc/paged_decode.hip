@@ -9,9 +9,12 @@
 // A lane leaves the first product with head lane % 16 and eight positions, which is the operand layout of
 // the second once the order of its K index is taken to be the order the lane holds. All rows are loaded whole,
 // past the caches: those of K are turned into operands through the wavefront's own part of LDS, those of V in
-// registers by byte permutes, so that product w yields the dims (dim / 16) m + w. The running maximum, the sum and the outputs of a head stay in the lanes of that head:
-// the maximum that weights refer to is moved only when a score exceeds it by 2^8, so that the outputs are
-// rarely rescaled; weights are rounded to BF16 for the second product, their sum is kept in FP32.
+// registers by byte permutes, so that product w yields the dims (dim / 16) m + w. The running maximum, the
+// sum and the outputs of a head stay in the lanes of that head: the maximum that weights refer to is moved only when a
+// score exceeds it by 2^8 (a published technique), so that the outputs are rarely rescaled. Sums, maxima and partials are
+// FP32. Weights are rounded to BF16 for the second product: the matrix instruction takes them in the type of V, and a
+// second BF16 part for the bits lost would double that product. It costs 1.05 to 1.4 times the distance from
+// the softmax in 64 bits that FP32 weights have behind the same rounding of the output.
 //
 // Measured, 64 query and 8 key-value heads of 128: 32 sequences of 2048 positions 44.5 us, 6.05 TB/s; 64 of 1 to
 // 16384 378 us, 6.0 TB/s; one of 131072 96 us, 5.6 TB/s (a copy of 2 GiB moves 4.9 TB/s, reads alone are faster);
@@ -19,7 +22,7 @@
 //
 // Work is divided by what the sequences hold, not by what the table could hold: all steps of a tile for each
 // wavefront (sequence, key-value head and 16 query heads, positions) are numbered and every workgroup takes an equal
-// run of them, so lengths may differ by any factor. A workgroup's wavefronts meet in LDS at the end of each
+// run of them, so lengths may differ by any factor (that it is divided at all goes by the table: decode_shares). A workgroup's wavefronts meet in LDS at the end of each
 // (sequence, heads); one that covered it whole writes the output, the others leave a partial (at most two
 // per workgroup) that a second kernel joins in order. Where the workgroups that one (sequence, heads) each
 // would make are enough, there are no partials and one launch.
@@ -514,7 +517,10 @@ template <int DIM> __global__ __launch_bounds__(JOIN_THREADS) void paged_decode_
 }
 } // namespace
 
-// How a call is divided: workgroups that share all steps, or 0 for one workgroup per (heads, sequence).
+// How a call is divided: workgroups that share all steps, or 0 for one workgroup per (heads, sequence). `positions` is what
+// the table has room for, or the window: the host does not see the lengths. A table that is wider than its sequences
+// are long makes short ones be shared too (64 query and 8 key-value heads of 128, table that fits / of 131072
+// positions: 1 sequence of 64 positions 5.2 / 9.0 us, 32 of 64 5.5 / 10.4, 32 of 1024 25.0 / 32.4, 32 of 2048 45.1 / 52.8).
 // Sharing costs a second launch and the numbering of the steps, some 4 us, and keeps every compute unit busy
 // whatever the lengths; one workgroup each is done when the longest sequence is. Measured, 64 query and 8
 // key-value heads of 128, whole / shared: 8 items of 512 positions 9.9 / 11.2 us, of 1024 15.4 / 11.2; 128 items of

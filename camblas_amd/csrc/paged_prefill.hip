@@ -16,14 +16,17 @@
 // row s / 4 of four rows, values 4 (s % 4) .. + 3, and receives the four values of column s).
 //
 // Rows of K and V go from memory into LDS directly, a tile ahead of the products. The maximum that weights
-// refer to is moved only when a score exceeds it by 2^8; weights are rounded to BF16 for the second product,
-// their sum is kept in FP32.
+// refer to is moved only when a score exceeds it by 2^8. Sums, maxima and partials are FP32; weights are rounded to
+// BF16 for the second product, whose matrix instruction takes them in the type of V (a second BF16 part for the bits
+// lost would double that product). It costs 1.3 to 1.4 times the distance from the softmax in 64 bits that FP32
+// weights have behind the same rounding of the output.
 //
-// Measured, 64 query and 8 key-value heads of 128: 2048 tokens after 30001 positions 1.90 ms, 1096 TFLOP/s; 4096 tokens
-// from the beginning 272 us, 1010 TFLOP/s (a large matrix product reaches 1410). Heads of 128 are bound by the power
-// that the matrix units may draw: those are busy 62 % of the cycles, at 1.7 to 1.8 GHz. Six prompts of 28 query and 4
-// key-value heads of 64 behind a window of 1024: 152 us, 665 TFLOP/s; the work on scores is the same for half the
-// products (matrix units busy 36 %, vector instructions issued in 72 % of the cycles).
+// Measured, 64 query and 8 key-value heads of 128: 2048 tokens after 30001 positions 1.87 to 2.01 ms from card to card,
+// 1036 to 1113 TFLOP/s; 4096 tokens from the beginning 270 to 284 us, 968 to 1018 TFLOP/s (a large matrix product reaches 1410).
+// Matrix units are busy 62 % and 57 % of the cycles, which run at 1.5 to 1.75 GHz under this load: both the clock and
+// the cycles without a matrix instruction bound them. Six prompts of 28 query and 4 key-value heads of 64 behind a window of
+// 1024: 145 to 154 us, 655 to 696 TFLOP/s; the work on scores is the same for half the products (matrix units busy 36 %,
+// vector instructions issued in 72 % of the cycles, at 1.85 GHz).
 #include "common.hpp"
 #include "device.hpp"
 #include "dma.hpp"
@@ -640,8 +643,10 @@ template <int DIM> __global__ __launch_bounds__(THREADS) void paged_prefill_join
 int64_t prefill_blocks(int batch, int tokens, int group) { return int64_t(tokens) * group / ROWS + batch; }
 
 // Over how many workgroups the positions of a block of rows are divided: as many as fill the chip where the
-// blocks alone do not, with a few tiles each. Measured, one workgroup / shares: 7 sequences of up to 41 tokens past
-// 2000 positions 56 / 27 us; 15 of one token past 7000 154 / 20; 64 tokens past 16000 389 / 57.
+// blocks alone do not, with a few tiles each, going by what the table has room for, or the window: the host does not see the
+// lengths. Measured, one workgroup / shares, before later steps: 7 sequences of up to 41 tokens past 2000 positions 56 / 27
+// us (24.5 now); 15 of one token past 7000 154 / 20; 64 tokens past 16000 389 / 57. Shares that hold no tile still leave
+// their partials (a table that fits / of 131072 positions: one prompt of 16 tokens 7.1 / 19.4 us, of 324 12.1 / 23.5).
 int prefill_shares(int64_t blocks, int dim, int64_t positions, int compute_units)
 {
     const int64_t room = int64_t(dim == 64 ? 3 : 2) * compute_units / (blocks > 0 ? blocks : 1);

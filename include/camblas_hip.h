@@ -399,8 +399,9 @@ int camblas_cuda_fp8_moe_decode(camblas_cuda_context *context, int experts, int 
  * A sequence's row of a page table (int32 [batch][table_columns], table_stride apart) maps its position p to
  * page table[p / page_size], slot p % page_size. Entries outside [0, pages) hold nothing: such positions are
  * neither read nor attended to. table_columns * page_size is at most 2^30; lengths are clipped to it. Query
- * rows times q_heads are at most 2^30, the tokens of one append 2^25. Rows that are written share no memory
- * with those that are read, except as stated. */
+ * rows times q_heads are at most 2^30, sequences 65535, the tokens of one append 2^25; in prefill, blocks of 128 rows
+ * (tokens * q_heads / kv_heads / 128 + batch) times kv_heads stay below 2^24. Rows that are written share no
+ * memory with those that are read, except as stated. */
 typedef struct camblas_cuda_paged_cache {
     void *k, *v;
     int64_t page_stride, slot_stride, head_stride;
@@ -434,8 +435,9 @@ int camblas_cuda_qk_norm_rope_append_wide_theta(camblas_cuda_context *context, i
  * second product, one rounding at the end; zeros where a token sees nothing (NaN where it sees positions whose scores are
  * all minus infinity: a softmax of 0 / 0). The cache's rows that a token does
  * not see do not reach its output, whatever they hold. workspace: ..._workspace_size() bytes (0: none), 16-byte
- * aligned, written before it is read; calls that may run at the same time need one each. No atomics: results repeat bit for
- * bit on one device. */
+ * aligned, written before it is read; calls that may run at the same time need one each. Nothing is summed by atomics:
+ * results repeat bit for bit on one device. How a call is divided goes by table_columns, or the window: rows of the
+ * table no longer than the sequences need make short ones up to twice as fast. */
 size_t camblas_cuda_paged_decode_workspace_size(const camblas_cuda_context *context, int batch, int q_heads,
                                                 const camblas_cuda_paged_cache *cache, int table_columns, int window,
                                                 int sinks);
